@@ -180,8 +180,10 @@ def _inputs(case, seed):
     elif case['spread'] == 'even':
         token = torch.randint(vocab, (tokens, ), generator=gen, device=DEVICE)
     else:
-        often = 1 / (2.7 + torch.randperm(vocab, generator=gen, device=DEVICE).float())
-        token = torch.multinomial(often, tokens, replacement=True, generator=gen)
+        # the r-th most frequent token about as often as 1 / (2.7 + r), element by element: no running sum, whose order
+        # (and with it a token here and there) could differ between two preparations
+        rank = 2.7 * ((1 + vocab / 2.7)**torch.rand(tokens, generator=gen, device=DEVICE, dtype=torch.float64) - 1)
+        token = torch.randperm(vocab, generator=gen, device=DEVICE)[rank.long().clamp(max=vocab - 1)]
     s = dict(token=token.to(getattr(torch, case['index'])).contiguous(), weight=(normal(vocab, width) * 0.02).to(dtype))
     if case['train']:
         s['dout'] = (normal(tokens, width) * 0.1).to(dtype)
