@@ -202,7 +202,8 @@ def prepare(case, seed):
             from elixir_b200 import kernels
             from elixir_b200.engine import ChunkStepEngine
             from elixir_b200.scaler import ConstantGradScaler
-            engine = ChunkStepEngine(DEVICE, _dtype(case), ConstantGradScaler(case['scale']), state_bits=8)
+            engine = ChunkStepEngine(torch.device(DEVICE, torch.cuda.current_device()), _dtype(case),
+                                     ConstantGradScaler(case['scale']), state_bits=8)
             for d in s['shards']:
                 engine.add_shard(d['master'], d['lowp'], d['valid'], [(a, b, g) for a, b, g in
                                                                       ((0, d['split'], 0), (d['split'], d['valid'], 1)) if a < b],
