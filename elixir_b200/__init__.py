@@ -3,8 +3,8 @@ NVIDIA B200 as hand-written sm_100a kernels behind a C ABI (``include/elixir_b20
 
 ``elixir_b200.kernels`` binds the ABI to torch tensors; ``elixir_b200.chunk`` and
 ``elixir_b200.wrapper`` mirror ``elixir.chunk`` and ``elixir.wrapper`` of the reference for this
-path.  Nothing here computes on the CPU: without the native library every operation raises.
+path; ``elixir_b200.functional`` holds operators of the wrapped model.  Nothing here computes on the CPU: without the native library every operation raises.
 """
-from . import _abi, _lib, kernels    # noqa: F401
+from . import _abi, _lib, functional, kernels    # noqa: F401
 
 __version__ = '0.1.0'

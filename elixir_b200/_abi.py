@@ -19,6 +19,8 @@ STAT_BAD_DESC = 2
 STAT_TIMEOUT = 4
 
 MAX_GROUPS = 64
+MOMENT_BLOCK = 256
+NORM_MAX_COLS = 1048576
 
 
 class ElxCtl(C.Structure):
@@ -162,6 +164,16 @@ PROTOTYPES = {
     'elx_adam_multi_pull_push': (_i, [_p, _i, _i, _i64, _i, _p, _p, _i, _p, ElxPeerTable, ElxPeerTable, _p, _p]),
     'elx_adam_chunk': (_i, [_p, _p, _p, _p, _i, _i64, _i64, ElxHyper, _p, _p]),
     'elx_cast_copyback': (_i, [_p, _p, _i, _i64, _p]),
+    'elx_moment_state_bytes': (_i64, [_i64]),
+    'elx_adam8_multi': (_i, [_p, _i, _i, _i64, _i, _p, _p, _i, _p, _p]),
+    'elx_moments_pack': (_i, [_p, _p, _i64, _p, _p, _p]),
+    'elx_moments_unpack': (_i, [_p, _p, _i64, _i, _p, _p, _p]),
+    'elx_layer_norm_forward': (_i, [_p, _p, _p, _i, _i64, _i64, _f, _p, _p, _p, _p]),
+    'elx_layer_norm_backward_workspace': (_i64, [_i64, _i64]),
+    'elx_layer_norm_backward': (_i, [_p, _p, _p, _p, _p, _i, _i64, _i64, _p, _p, _p, _p, _i64, _p]),
+    'elx_embedding_forward': (_i, [_p, _i, _i64, _p, _i, _i64, _i64, _f, _p, _p]),
+    'elx_embedding_backward_workspace': (_i64, [_i64, _i64]),
+    'elx_embedding_backward': (_i, [_p, _i, _i64, _p, _i, _i64, _i64, _f, _i64, _p, _p, _i64, _p]),
 }
 
 

@@ -13,6 +13,9 @@
 //   elx_probe.cu     inf/nan probe of the reduced low-precision gradients (optionally fused with the
 //                    copy into the shard, optionally with a fixed-order sum of squares)
 //   elx_peer.cu      NVLink: pull reduce-scatter fused with the probe, device-side barrier, IPC set-up
+//   elx_adam8.cu     the update with both moments in 8 bits (form: elx_moments.cuh) and their conversion
+//   elx_norm.cu      layer norm of the wrapped model, forward and backward
+//   elx_embed.cu     embedding lookup of the wrapped model and its gradient by sorted tokens
 //
 // Semantics follow hpcaitech/Elixir's ElixirOptimizer.step (elixir/wrapper/optimizer.py:192-220),
 // Chunk.update_extra_reduce_info / optim_update (elixir/chunk/core/chunk.py:345-356, 403-415) and

@@ -34,7 +34,11 @@ class ChunkStepEngine:
                  scaler: Optional[BaseGradScaler] = None,
                  process_group=None,
                  sync_overflow: bool = True,
-                 max_norm: float = 0.0):
+                 max_norm: float = 0.0,
+                 state_bits: int = 32):
+        """``state_bits=8`` holds both Adam moments in 8 bits (one byte per element each, a shared exponent byte per
+        256 elements) instead of fp32: 16 instead of 28 bytes of traffic per element and step.  For device-resident
+        shards and the steps that update in place (``step``, ``capture_step``, ``step_sharded``, ``step_from_host``)."""
         self.device = torch.device(device)
         self.dtype = dtype
         self.group = process_group
@@ -45,7 +49,8 @@ class ChunkStepEngine:
         self.clipping = max_norm > 0.0
         self.ctl = kernels.ControlBlock(self.device, self.scaler.initial_scale)
         self.scaler.attach(self.ctl)
-        self.table = kernels.ChunkTable(self.device, dtype)
+        self.state_bits = state_bits
+        self.table = kernels.ChunkTable(self.device, dtype, state_bits)
         self.shards: List[Tuple[torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor, int]] = []
         self.grad_srcs: List[Optional[torch.Tensor]] = []    # per shard: separate gradient source, or None
         self.chunk_flags: Optional[torch.Tensor] = None
@@ -73,8 +78,11 @@ class ChunkStepEngine:
         from ``lowp``, so that nothing has to be copied into the shard before the step (``probe`` instead of
         ``land``); ``lowp`` still receives the refreshed working copy.  The four arrays may also be
         pinned host tensors (a shard kept off the GPU): ``land``/``probe``/``step`` then reach them over PCIe
-        with the same kernels; the collective pipelines (``step_sharded*``) need device-resident shards."""
+        with the same kernels; the collective pipelines (``step_sharded*``) need device-resident shards.  With
+        8-bit moments the two moment arrays are state arrays (uint8, ``kernels.moment_state_bytes`` bytes)."""
         def zeros():    # where the master lives, page-locked if it is
+            if self.state_bits == 8:
+                return torch.zeros(kernels.moment_state_bytes(master.numel()), dtype=torch.uint8, device=master.device)
             return torch.zeros(master.shape, dtype=master.dtype, device=master.device,
                                pin_memory=kernels.is_mapped_host(master))
 
@@ -104,6 +112,21 @@ class ChunkStepEngine:
 
     def set_hyper(self, groups):
         self.table.set_hyper(groups)
+
+    def moments(self, index: int, dtype: torch.dtype = torch.float32) -> Tuple[torch.Tensor, torch.Tensor]:
+        """Both moments of shard ``index`` as numbers: the arrays themselves where they are fp32, copies in ``dtype``
+        (float32 or bfloat16) where the state is held in 8 bits."""
+        _, exp_avg, exp_avg_sq, lowp, _ = self.shards[index]
+        if self.state_bits != 8:
+            return exp_avg, exp_avg_sq
+        out = [torch.empty(lowp.numel(), dtype=dtype, device=exp_avg.device) for _ in range(2)]
+        kernels.unpack_moments(exp_avg, exp_avg_sq, *out)
+        return out[0], out[1]
+
+    def _need_fp32_moments(self, what: str):
+        if self.state_bits != 32:
+            raise RuntimeError(f'{what} works on fp32 moments; 8-bit moments are updated in place (step, step_sharded, '
+                               'step_from_host)')
 
     # ------------------------------------------------------------------ gradient arrival
 
@@ -308,6 +331,7 @@ class ChunkStepEngine:
         k uses block ``k % P`` — the regime of models whose replicated blocks cannot all be resident; the step
         then runs chunk by chunk (``step_sharded_p2p``).  ``grad_block(k)`` / ``gather_block(k)`` are this rank's
         blocks."""
+        self._need_fp32_moments('the peer-mapped step')
         from .peer import PeerBarrier, PeerBuffer
         assert len(chunk_sizes) == self.n_chunks
         for k, size in enumerate(chunk_sizes):
@@ -337,6 +361,7 @@ class ChunkStepEngine:
         offset ``block_offsets[k]``, holds that rank's gradients of chunk k before the step and receives the
         gathered parameters after it.  Rank r only ever reads and writes slice r of the other ranks' blocks, so
         sharing the slab between the two directions needs no extra ordering."""
+        self._need_fp32_moments('the peer-mapped step')
         from .peer import PeerBarrier
         assert len(block_offsets) == self.n_chunks
         self._p2p_pool = 0
@@ -635,6 +660,7 @@ class ChunkStepEngine:
         more) and its descriptor table.  ``step_single_pass`` / ``step_sharded_single_pass`` then read the current
         set and write the other one; which one is current is a word of the device control block, so the host never
         has to know (``current_shards`` reads it back for checkpoints and tests)."""
+        self._need_fp32_moments('the single-pass step')
         assert self.table.descs_dev is not None, 'finalize() first'
         if self._sets is not None:
             return self
@@ -691,6 +717,7 @@ class ChunkStepEngine:
         """Slabs for ``step_sharded_single_pass``: like ``enable_p2p`` (a gradient block and a gather block of
         ``chunk_sizes[k]`` elements per chunk on every rank), but in symmetric memory bound to an NVLink multicast
         object, so that the switch can add up the ranks' gradient blocks and deliver one store to all gather blocks."""
+        self._need_fp32_moments('the step through the switch')
         from .peer import PeerBarrier, SymmBuffer
         assert len(chunk_sizes) == self.n_chunks
         for k, size in enumerate(chunk_sizes):
@@ -873,6 +900,7 @@ class ChunkStepEngine:
     def enable_streaming(self, slots: int = 3):
         """Prepare ``step_streamed``: ``slots`` device staging sets (master, two moments, working copy) of the
         largest shard's size, and a second descriptor table whose entry k points into set ``k % slots``."""
+        self._need_fp32_moments('the streamed update')
         assert self.table.descs_dev is not None, 'finalize() first'
         assert self.table.host_resident, 'streaming is for shards kept in pinned host memory'
         size = max(s[0].numel() for s in self.shards)

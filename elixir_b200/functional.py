@@ -1,0 +1,122 @@
+"""Operators of the wrapped model with their gradients: layer norm, and the embedding lookup with a scale.
+
+``ElixirModule(use_fused_kernels=True)`` runs the ``nn.LayerNorm`` and ``nn.Embedding`` layers of its module through
+them (``use_kernels``), where the reference swaps in a fused layer norm (``elixir/kernels/layernorm.py:4``,
+``elixir/hook/parameter.py:69-70``).  Statistics and sums are fp32, every output is rounded once, and both parameter
+gradients are summed in an order that the inputs alone fix.  CUDA tensors only; first derivatives only.
+"""
+from functools import partial
+from typing import Optional
+
+import torch
+import torch.nn as nn
+from torch.autograd import Function
+from torch.autograd.function import once_differentiable
+
+from . import kernels
+
+_DTYPES = (torch.float16, torch.bfloat16, torch.float32)
+
+
+class _LayerNorm(Function):
+
+    @staticmethod
+    def forward(ctx, x, weight, bias, eps):
+        y, mean, rstd = kernels.layer_norm_forward(x, weight, bias, eps)
+        ctx.save_for_backward(x, weight, mean, rstd)
+        return y
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy):
+        x, weight, mean, rstd = ctx.saved_tensors
+        dx, dweight, dbias = kernels.layer_norm_backward(dy.contiguous(), x, weight, mean, rstd,
+                                                         weight_grad=ctx.needs_input_grad[1],
+                                                         bias_grad=ctx.needs_input_grad[2])
+        return dx if ctx.needs_input_grad[0] else None, dweight, dbias, None
+
+
+def layer_norm(x: torch.Tensor, normalized_shape, weight: Optional[torch.Tensor] = None,
+               bias: Optional[torch.Tensor] = None, eps: float = 1e-5) -> torch.Tensor:
+    """``torch.nn.functional.layer_norm`` on this package's kernels.  ``weight`` and ``bias`` have the type of ``x``."""
+    shape = (normalized_shape, ) if isinstance(normalized_shape, int) else tuple(normalized_shape)
+    if not shape or x.shape[-len(shape):] != shape or x.dim() < len(shape):
+        raise ValueError(f'normalized_shape {shape} does not end the shape {tuple(x.shape)}')
+    for name, t in (('weight', weight), ('bias', bias)):
+        if t is not None and t.shape != shape:
+            raise ValueError(f'{name} must have the shape {shape}')
+    flat = x.contiguous()
+    if len(shape) > 1:
+        flat = flat.flatten(-len(shape))
+        weight = None if weight is None else weight.contiguous().flatten()
+        bias = None if bias is None else bias.contiguous().flatten()
+    else:
+        weight = None if weight is None else weight.contiguous()
+        bias = None if bias is None else bias.contiguous()
+    return _LayerNorm.apply(flat, weight, bias, eps).view(x.shape)
+
+
+class _Embedding(Function):
+
+    @staticmethod
+    def forward(ctx, tokens, weight, padding_idx, scale):
+        ctx.save_for_backward(tokens)
+        ctx.vocab, ctx.padding_idx, ctx.scale = weight.shape[0], padding_idx, scale
+        return kernels.embedding_forward(tokens, weight, scale)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dout):
+        tokens, = ctx.saved_tensors
+        return None, kernels.embedding_backward(tokens, dout.contiguous(), ctx.vocab, ctx.scale, ctx.padding_idx), None, None
+
+
+def embedding(tokens: torch.Tensor, weight: torch.Tensor, padding_idx: Optional[int] = None, scale: float = 1.0) -> torch.Tensor:
+    """``scale * weight[tokens]``.  As with ``torch.nn.functional.embedding``, ``padding_idx`` (negative values count from
+    the end) names the token whose row gets no gradient; the gradient is dense.  A token outside the table, which torch
+    answers with a device assertion, reads as a row of NaN here: the overflow probe then skips the step."""
+    if padding_idx is not None:
+        if not -weight.shape[0] <= padding_idx < weight.shape[0]:
+            raise ValueError('padding_idx outside the table')
+        padding_idx %= weight.shape[0]
+    return _Embedding.apply(tokens.contiguous(), weight.contiguous(), padding_idx, float(scale))
+
+
+# ---------------------------------------------------------------------------------------------------
+# the layers of a module
+# ---------------------------------------------------------------------------------------------------
+
+
+def _plain_cuda(x, *params):
+    """The kernels take CUDA tensors of one supported type, outside autocast (which would change the types) and outside
+    torch's functional transforms."""
+    return (x.is_cuda and all(p is None or (p.is_cuda and p.dtype in _DTYPES and p.device == x.device) for p in params)
+            and not torch.is_autocast_enabled('cuda') and not torch._C._are_functorch_transforms_active())
+
+
+def _layer_norm_layer(layer: nn.LayerNorm, x):
+    if x.dtype in _DTYPES and all(p is None or p.dtype == x.dtype for p in (layer.weight, layer.bias)) and _plain_cuda(
+            x, layer.weight, layer.bias):
+        return layer_norm(x, layer.normalized_shape, layer.weight, layer.bias, layer.eps)
+    return nn.LayerNorm.forward(layer, x)
+
+
+def _embedding_layer(layer: nn.Embedding, tokens):
+    if (tokens.dtype in (torch.int32, torch.int64) and layer.max_norm is None and not layer.sparse
+            and not layer.scale_grad_by_freq and _plain_cuda(tokens, layer.weight)):
+        return embedding(tokens, layer.weight, layer.padding_idx)
+    return nn.Embedding.forward(layer, tokens)
+
+
+def use_kernels(module: nn.Module) -> int:
+    """Run every ``nn.LayerNorm`` and ``nn.Embedding`` of ``module`` (subclasses that keep their ``forward`` included)
+    through this package's kernels wherever those apply: CUDA tensors, one type for input and parameters, no autocast;
+    embeddings without ``max_norm``, ``sparse`` and ``scale_grad_by_freq``.  Other calls stay with torch.  Returns the
+    number of layers."""
+    count = 0
+    for layer in module.modules():
+        for kind, forward in ((nn.LayerNorm, _layer_norm_layer), (nn.Embedding, _embedding_layer)):
+            if isinstance(layer, kind) and type(layer).forward is kind.forward:
+                layer.forward = partial(forward, layer)
+                count += 1
+    return count

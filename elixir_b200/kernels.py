@@ -68,7 +68,8 @@ class _DeviceGuard:
     """Make the tensor's device current for the duration of a native call."""
 
     def __init__(self, t: Optional[torch.Tensor]):
-        self._ctx = torch.cuda.device(t.device) if (t is not None and t.is_cuda) else None
+        elsewhere = t is not None and t.is_cuda and t.device.index != torch.cuda.current_device()
+        self._ctx = torch.cuda.device(t.device) if elsewhere else None
 
     def __enter__(self):
         if self._ctx is not None:
@@ -313,11 +314,17 @@ class ChunkTable:
     ``add_chunk`` records a shard with its parameter segments; ``finalize`` uploads the descriptor
     and segment tables once; ``set_hyper`` uploads the (small) hyper-parameter table whenever a
     value changed, from a ring of pinned staging buffers so that no upload ever waits for the host.
+
+    ``state_bits=8``: ``exp_avg`` and ``exp_avg_sq`` are 8-bit state arrays (uint8, ``moment_state_bytes(n)`` bytes
+    each, zeros for a new optimizer) and ``adam_multi`` runs the update for them.
     """
 
     _RING = 4
 
-    def __init__(self, device, dtype: torch.dtype):
+    def __init__(self, device, dtype: torch.dtype, state_bits: int = 32):
+        if state_bits not in (8, 32):
+            raise ValueError(f'moments are held in 32 or in 8 bits, not in {state_bits}')
+        self.state_bits = state_bits
         self.device = torch.device(device)
         self.dtype = dtype
         self.code = dtype_code(dtype)
@@ -352,11 +359,16 @@ class ChunkTable:
         ``grad_param`` either way."""
         if self.descs_dev is not None:
             raise RuntimeError('the table is already finalized')
-        for name, t in (('master', master), ('exp_avg', exp_avg), ('exp_avg_sq', exp_avg_sq)):
-            _check_tensor(t, name, torch.float32, mapped_host=True)
+        if self.state_bits == 8 and not _lib.host_memory_backend():
+            if any(t is not None and not t.is_cuda for t in (master, exp_avg, exp_avg_sq, grad_param, grad_src)):
+                raise ValueError('a table with 8-bit moments takes device-resident shards only')
+        _check_tensor(master, 'master', torch.float32, mapped_host=True)
+        for name, t in (('exp_avg', exp_avg), ('exp_avg_sq', exp_avg_sq)):
+            _check_tensor(t, name, torch.float32 if self.state_bits == 32 else torch.uint8, mapped_host=True)
         _check_tensor(grad_param, 'grad_param', self.dtype, mapped_host=True)
         n = master.numel()
-        if not (exp_avg.numel() == exp_avg_sq.numel() == grad_param.numel() == n):
+        n_moment = n if self.state_bits == 32 else moment_state_bytes(n)
+        if not (exp_avg.numel() == exp_avg_sq.numel() == n_moment and grad_param.numel() == n):
             raise ValueError('master, moments and the low-precision shard differ in size')
         if not 0 <= n_valid <= n:
             raise ValueError('n_valid outside [0, n_shard]')
@@ -470,12 +482,18 @@ def adam_multi(table: ChunkTable, ctl: ControlBlock, first: int = 0, count: Opti
     if table.n_groups and table.hyper_dev is None:
         raise RuntimeError('set_hyper() before the first step')
     # shards in pinned host memory are updated in place over PCIe by the load/store variant of the kernel
-    entry, name = ((_lib.get().elx_adam_multi_hostmem, 'elx_adam_multi_hostmem') if table.host_resident else
-                   (_lib.get().elx_adam_multi, 'elx_adam_multi'))
+    name = ('elx_adam8_multi' if table.state_bits == 8 else
+            'elx_adam_multi_hostmem' if table.host_resident else 'elx_adam_multi')
+    entry = getattr(_lib.get(), name)
     with _DeviceGuard(table.descs_dev):
         _lib.check(
             entry(_ptr(table.descs_dev), first, count, table.tiles(first, count), table.code, _ptr(table.segs_dev),
                   _ptr(table.hyper_dev), table.n_groups, ctl.ptr, _stream(table.descs_dev)), name)
+
+
+def _need_fp32_moments(*tables: ChunkTable):
+    if any(t.state_bits != 32 for t in tables):
+        raise RuntimeError('this form of the update works on fp32 moments; a table with 8-bit moments goes through adam_multi')
 
 
 def adam_multi_shadow(table: ChunkTable, shadow: ChunkTable, ctl: ControlBlock, first: int = 0,
@@ -484,6 +502,7 @@ def adam_multi_shadow(table: ChunkTable, shadow: ChunkTable, ctl: ControlBlock, 
     master and moments into those of ``shadow`` (same shards, registered in the same order) and the refreshed
     working copy over the gradients as usual."""
     count = table.n_chunks - first if count is None else count
+    _need_fp32_moments(table, shadow)
     if table.descs_dev is None or shadow.descs_dev is None:
         raise RuntimeError('finalize() both tables first')
     if shadow.n_chunks != table.n_chunks or shadow.tile_begin != table.tile_begin:
@@ -522,6 +541,7 @@ def step_commit(ctl: ControlBlock, cfg: ElxScalerCfg, chunk_flags: Optional[torc
 
 
 def _check_two_sets(table: 'ChunkTable', other: 'ChunkTable'):
+    _need_fp32_moments(table, other)
     if table.descs_dev is None or other.descs_dev is None:
         raise RuntimeError('finalize() both tables first')
     if other.n_chunks != table.n_chunks or other.tile_begin != table.tile_begin:
@@ -599,6 +619,7 @@ def adam_multi_push(table: ChunkTable, ctl: ControlBlock, gather_table, block_of
     """Fused update whose refreshed low-precision tiles are also stored into every rank's gather slab
     (``elx_adam_multi_push``)."""
     count = table.n_chunks - first if count is None else count
+    _need_fp32_moments(table)
     if table.host_resident:
         raise RuntimeError('the update fused with the push all-gather runs on device-resident shards only')
     _check_tensor(block_off, 'block_off', torch.int64)
@@ -617,6 +638,7 @@ def adam_multi_pull_push(table: ChunkTable, ctl: ControlBlock, grads_table, gath
     """Reduce-scatter, in-place update and all-gather in one launch over peer-mapped slabs
     (``elx_adam_multi_pull_push``); the decision must already exist."""
     count = table.n_chunks - first if count is None else count
+    _need_fp32_moments(table)
     if table.host_resident:
         raise RuntimeError('the update fused with both collectives runs on device-resident shards only')
     _check_tensor(block_off, 'block_off', torch.int64)
@@ -643,3 +665,181 @@ def copy_async(dst_ptr: int, src_ptr: int, nbytes: int, stream: torch.cuda.Strea
     """One copy-engine transfer between raw device addresses (local or peer-mapped) on ``stream``."""
     _lib.check(_lib.get().elx_copy_async(ctypes.c_void_p(dst_ptr), ctypes.c_void_p(src_ptr), nbytes,
                                          ctypes.c_void_p(stream.cuda_stream)), 'elx_copy_async')
+
+
+# ---------------------------------------------------------------------------------------------------
+# moments in 8 bits
+# ---------------------------------------------------------------------------------------------------
+
+
+def moment_state_bytes(n: int) -> int:
+    """Size of the 8-bit state array of one moment of a shard of ``n`` elements."""
+    return (n + 15) // 16 * 16 + ((n + _abi.MOMENT_BLOCK - 1) // _abi.MOMENT_BLOCK + 15) // 16 * 16
+
+
+def _same_device(*named):
+    home = named[0][1]
+    for name, t in named[1:]:
+        if t is not None and t.device != home.device:
+            raise ValueError(f'{name} is on {t.device}, {named[0][0]} on {home.device}')
+
+
+def pack_moments(exp_avg: torch.Tensor, exp_avg_sq: torch.Tensor, state_m: Optional[torch.Tensor] = None,
+                 state_v: Optional[torch.Tensor] = None) -> Tuple[torch.Tensor, torch.Tensor]:
+    """The fp32 moments of a shard in the 8-bit form, rounded to nearest (``elx_moments_pack``).  Returns the two state
+    arrays, the given ones or new ones."""
+    _check_tensor(exp_avg, 'exp_avg', torch.float32)
+    _check_tensor(exp_avg_sq, 'exp_avg_sq', torch.float32)
+    n = exp_avg.numel()
+    if exp_avg_sq.numel() != n:
+        raise ValueError('the two moments differ in size')
+    size = moment_state_bytes(n)
+    if state_m is None:
+        state_m = torch.zeros(size, dtype=torch.uint8, device=exp_avg.device)
+    if state_v is None:
+        state_v = torch.zeros(size, dtype=torch.uint8, device=exp_avg.device)
+    for name, t in (('state_m', state_m), ('state_v', state_v)):
+        _check_tensor(t, name, torch.uint8)
+        if t.numel() != size:
+            raise ValueError(f'{name} must hold moment_state_bytes({n}) = {size} bytes')
+    _same_device(('exp_avg', exp_avg), ('exp_avg_sq', exp_avg_sq), ('state_m', state_m), ('state_v', state_v))
+    if n:
+        with _DeviceGuard(exp_avg):
+            _lib.check(_lib.get().elx_moments_pack(_ptr(exp_avg), _ptr(exp_avg_sq), n, _ptr(state_m), _ptr(state_v),
+                                                   _stream(exp_avg)), 'elx_moments_pack')
+    return state_m, state_v
+
+
+def unpack_moments(state_m: torch.Tensor, state_v: torch.Tensor, exp_avg: torch.Tensor, exp_avg_sq: torch.Tensor):
+    """The values that two 8-bit state arrays stand for, into fp32 or bf16 tensors of the shard's size
+    (``elx_moments_unpack``)."""
+    _check_tensor(exp_avg, 'exp_avg')
+    if exp_avg.dtype not in (torch.float32, torch.bfloat16):
+        raise TypeError(f'moments are read out as float32 or bfloat16, not {exp_avg.dtype}')
+    _check_tensor(exp_avg_sq, 'exp_avg_sq', exp_avg.dtype)
+    n = exp_avg.numel()
+    if exp_avg_sq.numel() != n:
+        raise ValueError('the two moments differ in size')
+    for name, t in (('state_m', state_m), ('state_v', state_v)):
+        _check_tensor(t, name, torch.uint8)
+        if t.numel() != moment_state_bytes(n):
+            raise ValueError(f'{name} must hold moment_state_bytes({n}) = {moment_state_bytes(n)} bytes')
+    _same_device(('exp_avg', exp_avg), ('exp_avg_sq', exp_avg_sq), ('state_m', state_m), ('state_v', state_v))
+    if n:
+        with _DeviceGuard(exp_avg):
+            _lib.check(_lib.get().elx_moments_unpack(_ptr(state_m), _ptr(state_v), n, dtype_code(exp_avg.dtype), _ptr(exp_avg),
+                                                     _ptr(exp_avg_sq), _stream(exp_avg)), 'elx_moments_unpack')
+
+
+# ---------------------------------------------------------------------------------------------------
+# operators of the wrapped model
+# ---------------------------------------------------------------------------------------------------
+
+
+def _check_norm(x, weight, bias):
+    _check_tensor(x, 'x')
+    if x.dim() < 1 or x.shape[-1] < 1:
+        raise ValueError('x needs a last dimension of at least one element')
+    cols = x.shape[-1]
+    if cols > _abi.NORM_MAX_COLS:
+        raise ValueError(f'at most {_abi.NORM_MAX_COLS} elements per row are supported')
+    for name, t in (('weight', weight), ('bias', bias)):
+        if t is not None:
+            _check_tensor(t, name, x.dtype)
+            if t.numel() != cols:
+                raise ValueError(f'{name} must have {cols} elements')
+    _same_device(('x', x), ('weight', weight), ('bias', bias))
+    return x.numel() // cols, cols
+
+
+def layer_norm_forward(x: torch.Tensor, weight: Optional[torch.Tensor] = None, bias: Optional[torch.Tensor] = None,
+                       eps: float = 1e-5) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    """Layer norm over the last dimension of ``x`` (``elx_layer_norm_forward``).  Returns ``y`` and, per row and in
+    fp32, the mean and the reciprocal standard deviation that ``layer_norm_backward`` takes."""
+    rows, cols = _check_norm(x, weight, bias)
+    y = torch.empty_like(x)
+    stats = torch.empty((2, rows), dtype=torch.float32, device=x.device)
+    mean, rstd = stats[0], stats[1]
+    if rows:
+        with _DeviceGuard(x):
+            _lib.check(_lib.get().elx_layer_norm_forward(_ptr(x), _ptr(weight), _ptr(bias), dtype_code(x.dtype), rows, cols,
+                                                         eps, _ptr(y), _ptr(mean), _ptr(rstd), _stream(x)),
+                       'elx_layer_norm_forward')
+    return y, mean, rstd
+
+
+def layer_norm_backward(dy: torch.Tensor, x: torch.Tensor, weight: Optional[torch.Tensor], mean: torch.Tensor,
+                        rstd: torch.Tensor, weight_grad: bool = True, bias_grad: bool = True):
+    """``(dx, dweight, dbias)`` of ``layer_norm_forward`` (``elx_layer_norm_backward``).  ``dweight`` is None without a
+    weight or ``weight_grad``, ``dbias`` without ``bias_grad``."""
+    rows, cols = _check_norm(x, weight, None)
+    _check_tensor(dy, 'dy', x.dtype)
+    if dy.shape != x.shape:
+        raise ValueError('dy and x differ in shape')
+    for name, t in (('mean', mean), ('rstd', rstd)):
+        _check_tensor(t, name, torch.float32)
+        if t.numel() != rows:
+            raise ValueError(f'{name} must have one element per row')
+    _same_device(('x', x), ('dy', dy), ('mean', mean), ('rstd', rstd))
+    lib = _lib.get()
+    dx = torch.empty_like(x)
+    dweight = torch.empty(cols, dtype=x.dtype, device=x.device) if weight_grad and weight is not None else None
+    dbias = torch.empty(cols, dtype=x.dtype, device=x.device) if bias_grad else None
+    space, size = None, 0
+    if dweight is not None or dbias is not None:
+        size = lib.elx_layer_norm_backward_workspace(rows, cols)
+        space = torch.empty(max(size, 16), dtype=torch.uint8, device=x.device)
+    with _DeviceGuard(x):
+        _lib.check(lib.elx_layer_norm_backward(_ptr(dy), _ptr(x), _ptr(weight), _ptr(mean), _ptr(rstd), dtype_code(x.dtype), rows,
+                                               cols, _ptr(dx), _ptr(dweight), _ptr(dbias), _ptr(space), size, _stream(x)),
+                   'elx_layer_norm_backward')
+    return dx, dweight, dbias
+
+
+def _check_tokens(tokens):
+    _check_tensor(tokens, 'tokens')
+    if tokens.dtype not in (torch.int32, torch.int64):
+        raise TypeError(f'tokens must be int32 or int64, got {tokens.dtype}')
+
+
+def embedding_forward(tokens: torch.Tensor, weight: torch.Tensor, scale: float = 1.0) -> torch.Tensor:
+    """``scale * weight[tokens]`` (``elx_embedding_forward``), of shape ``tokens.shape + (width,)``.  A token outside the
+    table reads as a row of NaN."""
+    _check_tokens(tokens)
+    _check_tensor(weight, 'weight')
+    if weight.dim() != 2 or weight.numel() == 0:
+        raise ValueError('weight must be a table of at least one row and one column')
+    _same_device(('weight', weight), ('tokens', tokens))
+    code = dtype_code(weight.dtype)
+    out = torch.empty(tokens.shape + weight.shape[1:], dtype=weight.dtype, device=weight.device)
+    if tokens.numel():
+        with _DeviceGuard(weight):
+            _lib.check(_lib.get().elx_embedding_forward(_ptr(tokens), tokens.element_size(), tokens.numel(), _ptr(weight), code,
+                                                        weight.shape[0], weight.shape[1], scale, _ptr(out), _stream(weight)),
+                       'elx_embedding_forward')
+    return out
+
+
+def embedding_backward(tokens: torch.Tensor, dout: torch.Tensor, vocab: int, scale: float = 1.0,
+                       padding_idx: Optional[int] = None) -> torch.Tensor:
+    """The dense gradient of ``embedding_forward`` with respect to a table of ``vocab`` rows
+    (``elx_embedding_backward``).  Tokens equal to ``padding_idx`` or outside the table add to no row."""
+    _check_tokens(tokens)
+    _check_tensor(dout, 'dout')
+    if dout.dim() < 1 or dout.shape[:-1] != tokens.shape or dout.shape[-1] < 1:
+        raise ValueError('dout must have the shape of tokens and one more dimension')
+    if vocab < 1:
+        raise ValueError('the table needs at least one row')
+    if padding_idx is not None and not 0 <= padding_idx < vocab:
+        raise ValueError('padding_idx outside the table')
+    _same_device(('dout', dout), ('tokens', tokens))
+    code, width, n = dtype_code(dout.dtype), dout.shape[-1], tokens.numel()
+    lib = _lib.get()
+    dweight = torch.empty((vocab, width), dtype=dout.dtype, device=dout.device)
+    size = lib.elx_embedding_backward_workspace(n, width)
+    space = torch.empty(max(size, 16), dtype=torch.uint8, device=dout.device)
+    with _DeviceGuard(dout):
+        _lib.check(lib.elx_embedding_backward(_ptr(tokens), tokens.element_size(), n, _ptr(dout), code, vocab, width, scale,
+                                              -1 if padding_idx is None else padding_idx, _ptr(dweight), _ptr(space), size,
+                                              _stream(dout)), 'elx_embedding_backward')
+    return dweight

@@ -24,10 +24,15 @@ class ChunkAdam(torch.optim.Optimizer):
                  eps: float = 1e-8,
                  weight_decay: float = 0,
                  adamw_mode: bool = True,
+                 state_bits: int = 32,
                  **unused):
+        """``state_bits=8``: both moments in 8 bits instead of fp32 (a block of 256 elements shares an exponent byte)."""
+        if state_bits not in (8, 32):
+            raise ValueError(f'moments are held in 32 or in 8 bits, not in {state_bits}')
         defaults = dict(lr=lr, bias_correction=bias_correction, betas=betas, eps=eps, weight_decay=weight_decay)
         super().__init__(model_params, defaults)
         self.adamw_mode = adamw_mode
+        self.state_bits = state_bits
         self._engine = None
 
     def bind_engine(self, engine):

@@ -38,7 +38,7 @@ import torch
 import torch.distributed as dist
 import torch.nn as nn
 
-from .. import comm
+from .. import comm, functional
 from ..chunk import ChunkFetcher, ChunkGroup, FIFOScheduler, MemoryPool, PrefetchScheduler, TensorState
 from .plan import SearchResult
 
@@ -86,7 +86,8 @@ class ElixirModule(nn.Module):
                  residency: Optional[str] = None) -> None:
         """Arguments as ``elixir.wrapper.ElixirModule`` (``module.py:40-48``).  ``residency`` (not in the
         reference): ``'all'``, ``'scheduled'`` or None = scheduled exactly when the replica cache has fewer
-        public blocks than there are public chunks."""
+        public blocks than there are public chunks.  ``use_fused_kernels``: the module's ``nn.LayerNorm`` and
+        ``nn.Embedding`` layers run this package's kernels on CUDA tensors (the reference swaps its layer norm)."""
         super().__init__()
         # the reference accepts float and float16 (module.py:51); bfloat16 is an extension that runs with
         # a constant loss scale of 1
@@ -136,6 +137,8 @@ class ElixirModule(nn.Module):
             param.register_post_accumulate_grad_hook(landed)
         if self.scheduled:
             self._install_residency_hooks()
+        if use_fused_kernels:
+            functional.use_kernels(module)
 
     # ------------------------------------------------------------------ construction
 

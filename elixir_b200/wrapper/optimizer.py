@@ -22,6 +22,7 @@ from typing import Dict, List, Set, Tuple
 import torch
 from torch.nn import Parameter
 
+from .. import kernels
 from ..chunk import Chunk
 from ..engine import ChunkStepEngine
 from ..optim import FusedAdam, HybridAdam
@@ -122,8 +123,11 @@ class ElixirOptimizer:
         device = chunks[0].compute_device if chunks else torch.device('cuda', torch.cuda.current_device())
         dtype = self.module.dtype
         group = self.module.process_group
+        state_bits = self.optim.state_bits if self.scaled_optimizer else 32
+        if state_bits == 8 and self.module.nvlink_step:
+            raise ValueError('the NVLink step works on fp32 moments; 8-bit moments need a plan without peer_group')
         self.engine = ChunkStepEngine(device, dtype, self.grad_scaler, process_group=group,
-                                      sync_overflow=sync_overflow, max_norm=self.max_norm)
+                                      sync_overflow=sync_overflow, max_norm=self.max_norm, state_bits=state_bits)
         for chunk in chunks:
             master = chunk.paired_chunk.shard
             # a foreign optimizer keeps its own state: no flat moments are allocated for it (the master stands in
@@ -145,8 +149,12 @@ class ElixirOptimizer:
             return
         self.optim.bind_engine(self.engine)
         self.engine.set_hyper(self.optim.hyper_table())
-        # per-parameter views of the flat moments, under the keys the reference's optimizers use
+        # per-parameter views of the flat moments, under the keys the reference's optimizers use (8-bit moments have no
+        # such views: engine.moments(i) reads a shard's out)
         for fake, (begin, end) in self.param_to_range.items():
+            if state_bits == 8:
+                self.optim.state[fake] = dict(step=0)
+                continue
             _, exp_avg, exp_avg_sq, _, _ = self.engine.shards[self._index_of[self.param_to_optim_chunk[fake]]]
             self.optim.state[fake] = dict(step=0, exp_avg=exp_avg[begin:end], exp_avg_sq=exp_avg_sq[begin:end])
 
@@ -284,7 +292,8 @@ class ElixirOptimizer:
 
     def state_dict(self):
         """This rank's flat optimizer state: one (exp_avg, exp_avg_sq) pair per chunk shard plus the control
-        block fields.  The reference saves none of this (its scaler state is lost on restart)."""
+        block fields.  The reference saves none of this (its scaler state is lost on restart).  8-bit moments are
+        saved as they are held; ``load_state_dict`` takes moments saved in either form."""
         self._quiesce_host_shards()
         self.engine.check_status()
         if not self.scaled_optimizer:
@@ -301,6 +310,23 @@ class ElixirOptimizer:
         if self.engine.table.host_resident:
             torch.cuda.synchronize(self.engine.device)
 
+    def _load_moments(self, shard, exp_avg, exp_avg_sq):
+        """Moments saved in either form into this optimizer's form."""
+        if exp_avg.dtype == shard[1].dtype:
+            shard[1].copy_(exp_avg)
+            shard[2].copy_(exp_avg_sq)
+        elif self.engine.state_bits == 8:
+            device = shard[1].device
+            kernels.pack_moments(exp_avg.to(device), exp_avg_sq.to(device), shard[1], shard[2])
+        elif shard[1].device == self.engine.device:
+            device = shard[1].device
+            kernels.unpack_moments(exp_avg.to(device), exp_avg_sq.to(device), shard[1], shard[2])
+        else:    # moments in host memory: converted on the device first
+            out = [torch.empty(shard[1].shape, device=self.engine.device) for _ in range(2)]
+            kernels.unpack_moments(exp_avg.to(self.engine.device), exp_avg_sq.to(self.engine.device), *out)
+            shard[1].copy_(out[0])
+            shard[2].copy_(out[1])
+
     def load_state_dict(self, state):
         self._quiesce_host_shards()
         self.grad_scaler.load_state_dict(state['scaler'])
@@ -308,7 +334,6 @@ class ElixirOptimizer:
             self.optim.load_state_dict(state['optim'])
             return
         for shard, saved in zip(self.engine.shards, state['shards']):
-            shard[1].copy_(saved['exp_avg'])
-            shard[2].copy_(saved['exp_avg_sq'])
+            self._load_moments(shard, saved['exp_avg'], saved['exp_avg_sq'])
         for group, saved in zip(self.optim.param_groups, state['param_groups']):
             group.update(saved)

@@ -511,6 +511,83 @@ int elx_adam_chunk(float* master, float* exp_avg, float* exp_avg_sq, void* grad_
  * Replaces Chunk.optim_update for CUDA shards (chunk.py:413-415). */
 int elx_cast_copyback(const float* master, void* dst, int dtype, int64_t n, void* stream);
 
+/* ---- the update with both moments in 8 bits ---------------------------------------------------- */
+
+/*
+ * State array of one moment of a shard of n elements: n one-byte codes, then, from the next multiple of 16 bytes, one
+ * exponent byte E per block of ELX_MOMENT_BLOCK elements (all zero bytes = all moments zero).  A code holds a small
+ * float relative to 2^(E - 127): the first moment a sign, 4 exponent bits f and 3 mantissa bits t, the second moment 5
+ * exponent bits and 3 mantissa bits; f > 0: (1 + t/8) 2^(f - F), f = 0: t/8 2^(1 - F), with F = 15 and 31.  E = 0: the
+ * block is zero; E = 255: it held an inf or a NaN and every element reads as NaN.  The largest magnitude is 1.875 2^126;
+ * what is above is held as that.
+ * elx_moment_state_bytes: size of that array (a negative ELX_ERR_SIZE for n < 0).
+ */
+#define ELX_MOMENT_BLOCK 256
+int64_t elx_moment_state_bytes(int64_t n);
+
+/*
+ * elx_adam_multi with both moments in 8 bits: 16 bytes per element with 16-bit gradients instead of 28, and 2 bytes of
+ * moments per element of memory instead of 8.  Same arguments, decision and results in the control block; in the
+ * descriptors exp_avg and exp_avg_sq point to state arrays (elx_moment_state_bytes(n_shard) bytes each, device memory).
+ * The new moments are formed in fp32, the parameter moves by them as they are, and they are stored with stochastic
+ * rounding: the rounding bits are a function of ctl->step, the descriptor's index in the table and the element's place
+ * in the shard, so the result is the same for every launch shape and for every split of the table into launches, and
+ * the expected value of a stored moment is the moment itself.  A second moment above zero is never stored as zero.
+ * In a block of which only a part lies inside segments the other elements keep the values of their moments (re-coded
+ * where the block's exponent changes); a block outside all segments is left as it is.  A skipped step refreshes the
+ * working copies only.  Root and division of the parameter's step are approximate (within 1e-6 relative); "math_mode"
+ * does not apply.  All pointers of a descriptor should be 32-byte aligned; other alignments are handled element by
+ * element.
+ */
+int elx_adam8_multi(const ElxChunkDesc* descs, int first, int count, int64_t n_tiles, int dtype, const ElxSeg* segs,
+                    const ElxHyper* hyper, int n_groups, ElxCtl* ctl, void* stream);
+
+/*
+ * Both moments of a shard into the 8-bit form (rounded to nearest) and back.  exp_avg, exp_avg_sq: device, n floats
+ * (unpack: n elements of `dtype`, ELX_F32 or ELX_BF16; bf16 holds every value from 2^-126 up exactly).  state_m,
+ * state_v: device, elx_moment_state_bytes(n) bytes; pack leaves the padding bytes as they are.  The sign of exp_avg_sq
+ * is dropped.  For checkpoints that hold fp32 moments, and for readers of the state.
+ */
+int elx_moments_pack(const float* exp_avg, const float* exp_avg_sq, int64_t n, void* state_m, void* state_v, void* stream);
+int elx_moments_unpack(const void* state_m, const void* state_v, int64_t n, int dtype, void* exp_avg, void* exp_avg_sq,
+                       void* stream);
+
+/* ---- operators of the wrapped model ------------------------------------------------------------- */
+
+/*
+ * Layer norm over the last dimension of x[rows][cols] (row-major, no gaps), every array of type `dtype`:
+ *   y = (x - mean) rstd weight + bias,  rstd = 1 / sqrt(mean((x - mean)^2) + eps)
+ * Statistics and sums in fp32, one rounding per output.  mean, rstd: device, `rows` floats, kept for the backward pass.
+ * weight, bias: `cols` elements or NULL (1 and 0).  Arrays need the alignment of their element; 16-byte accesses are
+ * used when every row starts on a 16-byte boundary.  rows = 0 is allowed; 1 <= cols <= ELX_NORM_MAX_COLS.
+ * elx_layer_norm_backward: dx, and the sums over the rows dweight = sum dy xhat and dbias = sum dy (each `cols`
+ * elements, NULL = not wanted), in an order that depends on rows and cols alone.  The sums need a workspace of
+ * elx_layer_norm_backward_workspace(rows, cols) bytes, 16-byte aligned, not shared with a call that may run at the
+ * same time; without them it may be NULL.  dx must not overlap the inputs.
+ */
+#define ELX_NORM_MAX_COLS 1048576
+int elx_layer_norm_forward(const void* x, const void* weight, const void* bias, int dtype, int64_t rows, int64_t cols,
+                           float eps, void* y, float* mean, float* rstd, void* stream);
+int64_t elx_layer_norm_backward_workspace(int64_t rows, int64_t cols);
+int elx_layer_norm_backward(const void* dy, const void* x, const void* weight, const float* mean, const float* rstd, int dtype,
+                            int64_t rows, int64_t cols, void* dx, void* dweight, void* dbias, void* workspace,
+                            int64_t workspace_bytes, void* stream);
+
+/*
+ * Embedding lookup out[i] = scale * weight[tokens[i]] (product in fp32, rounded once) for n tokens of index_bytes (4 or
+ * 8, signed) bytes each, and its gradient dweight[v] = scale * sum of dout[i] over the i with tokens[i] == v: dense,
+ * every row written, zero where no token points.  The sum is fp32, in ascending order within pieces whose borders the
+ * tokens alone fix, so it is the same for every run.  Tokens equal to padding_idx (-1 = none) add to no row.  A token
+ * outside [0, vocab) reads as a row of NaN and adds to no row.  workspace: elx_embedding_backward_workspace(n, width)
+ * bytes, 16-byte aligned, not shared with a call that may run at the same time.
+ */
+int elx_embedding_forward(const void* tokens, int index_bytes, int64_t n, const void* weight, int dtype, int64_t vocab,
+                          int64_t width, float scale, void* out, void* stream);
+int64_t elx_embedding_backward_workspace(int64_t n, int64_t width);
+int elx_embedding_backward(const void* tokens, int index_bytes, int64_t n, const void* dout, int dtype, int64_t vocab,
+                           int64_t width, float scale, int64_t padding_idx, void* dweight, void* workspace,
+                           int64_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

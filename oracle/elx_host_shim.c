@@ -7,6 +7,7 @@
  * argument is ignored, every call completes before it returns.  Arithmetic: elx_oracle.c (double
  * precision evaluation of the update, rounded to fp32).
  */
+#include <math.h>
 #include <stdint.h>
 #include <string.h>
 
@@ -416,4 +417,214 @@ int elx_copy_async(void* dst, const void* src, int64_t bytes, void* stream) {
     if (!dst || !src) return ELX_ERR_NULL;
     memmove(dst, src, (size_t)bytes);
     return ELX_OK;
+}
+
+/* ---- the update with both moments in 8 bits ---- */
+
+static float bits_f32(uint32_t u) {
+    float f;
+    memcpy(&f, &u, 4);
+    return f;
+}
+static uint32_t f32_bits(float f) {
+    uint32_t u;
+    memcpy(&u, &f, 4);
+    return u;
+}
+static int64_t exps_at(int64_t n) { return (n + 15) / 16 * 16; }
+static int64_t blocks_of(int64_t n) { return (n + ELX_MOMENT_BLOCK - 1) / ELX_MOMENT_BLOCK; }
+
+int64_t elx_moment_state_bytes(int64_t n) { return n < 0 ? ELX_ERR_SIZE : exps_at(n) + (blocks_of(n) + 15) / 16 * 16; }
+
+static double pow2(int e) { return ldexp(1.0, e); }
+
+/* value of a code; `first`: the signed moment */
+static float code_value(uint8_t c, uint8_t e, int first) {
+    if (e == 255) return bits_f32(0x7FC00000u);
+    if (e == 0) return 0.0f;
+    const int bias = first ? 15 : 31, mag = first ? c & 127 : c, f = mag >> 3, t = mag & 7;
+    const double v = f ? (1.0 + t / 8.0) * pow2(f - bias) : t / 8.0 * pow2(1 - bias);
+    const float x = (float)(v * pow2((int)e - 127));
+    return first && (c & 128) ? -x : x;
+}
+
+static uint8_t block_exp(const float* x, int n) {
+    uint32_t top = 0;
+    for (int i = 0; i < n; ++i) {
+        const uint32_t u = f32_bits(x[i]) & 0x7FFFFFFFu;
+        if (u > top) top = u;
+    }
+    if (top >= 0x7F800000u) return 255;
+    if (top == 0) return 0;
+    uint32_t e = (top + 0xFFFFFu) >> 23;
+    return (uint8_t)(e < 1 ? 1 : e > 253 ? 253 : e);
+}
+
+/* `up` in [0, 1): how far towards the next code a value is pushed before the fraction is dropped (0.5: nearest) */
+static uint8_t code_of(float x, uint8_t e, int first, double up) {
+    const int bias = first ? 15 : 31, top = first ? 127 : 255, sign = first && (f32_bits(x) >> 31) ? 128 : 0;
+    if (e == 0 || e == 255) return (uint8_t)sign;
+    const double a = fabs((double)x) / pow2((int)e - 127);
+    int f = bias;                                        /* exponent field of the binade that holds a (1: or below) */
+    while (f > 1 && a < pow2(f - bias)) --f;
+    /* in codes, counted from the foot of the binade's own spacing: 23 bits are held, the lowest 20 are dropped */
+    const double units = floor(a / pow2(f - bias - 23)) / 1048576.0;
+    int c = (int)(units + up) + (f - 1) * 8;
+    if (c > top) c = top;
+    if (!first && x > 0.0f && c < 1) c = 1;
+    return (uint8_t)(c | sign);
+}
+
+static uint32_t mix(uint32_t x) {
+    x = (x ^ (x >> 16)) * 0x9E3779B1u;
+    x = (x ^ (x >> 15)) * 0x85157AF5u;
+    return x ^ (x >> 16);
+}
+
+static void adam8_shard(const ElxChunkDesc* d, int index, const ElxSeg* segs, const ElxHyper* hyper, int n_groups,
+                        const ElxCtl* ctl) {
+    uint8_t *sm = (uint8_t*)d->exp_avg, *sv = (uint8_t*)d->exp_avg_sq;
+    uint8_t *em = sm + exps_at(d->n_shard), *ev = sv + exps_at(d->n_shard);
+    for (int64_t b = 0; b < blocks_of(d->n_shard) && !ctl->skip; ++b) {
+        const int64_t e0 = b * ELX_MOMENT_BLOCK;
+        const int len = (int)(d->n_shard - e0 < ELX_MOMENT_BLOCK ? d->n_shard - e0 : ELX_MOMENT_BLOCK);
+        float m[ELX_MOMENT_BLOCK], v[ELX_MOMENT_BLOCK];
+        int touched = 0;
+        for (int i = 0; i < len; ++i) {
+            m[i] = code_value(sm[e0 + i], em[b], 1);
+            v[i] = code_value(sv[e0 + i], ev[b], 0);
+        }
+        for (int s = d->seg_first; s < d->seg_first + d->seg_count; ++s) {
+            if (segs[s].group < 0 || segs[s].group >= n_groups) continue;
+            const ElxHyper h = hyper[segs[s].group];
+            for (int64_t e = segs[s].begin > e0 ? segs[s].begin : e0; e < segs[s].end && e < e0 + len; ++e) {
+                const int i = (int)(e - e0);
+                const float om1 = 1.0f - h.beta1, om2 = 1.0f - h.beta2;
+                const void* src = grad_of(d);
+                float g = d->dtype == ELX_F32    ? ((const float*)src)[e]
+                          : d->dtype == ELX_F16 ? orc_f16_to_f32(((const uint16_t*)src)[e])
+                                                : orc_bf16_to_f32(((const uint16_t*)src)[e]);
+                if (ctl->div_scale > 0.0f) g = g / ctl->div_scale;
+                const float p = d->master[e];
+                if (!h.adamw_mode) g = (float)((double)h.weight_decay * p + (double)g);
+                const float m1 = h.beta1 * m[i], m2 = om1 * g, v1 = h.beta2 * v[i], v2 = om2 * g, v3 = v2 * g;
+                m[i] = m1 + m2;
+                v[i] = v1 + v3;
+                /* the parameter's own step, in double */
+                double bc1 = 1.0, bc2 = 1.0;
+                if (h.bias_correction) {
+                    double t1 = 1.0, t2 = 1.0;
+                    for (int t = 0; t < ctl->step; ++t) {
+                        t1 *= h.beta1;
+                        t2 *= h.beta2;
+                    }
+                    bc1 -= t1;
+                    bc2 -= t2;
+                }
+                double upd = m[i] / bc1 / (sqrt(v[i] / bc2) + h.eps);
+                if (h.adamw_mode) upd += (double)h.weight_decay * p;
+                d->master[e] = (float)(p - h.lr * upd);
+                touched = 1;
+            }
+        }
+        if (!touched) continue;
+        em[b] = block_exp(m, len);
+        ev[b] = block_exp(v, len);
+        uint32_t key = mix((uint32_t)ctl->step * 0x632BE5ABu + (uint32_t)index * 0x9E3779B1u + 0x2545F491u);
+        key = mix(mix(key ^ (uint32_t)b) ^ (uint32_t)((uint64_t)b >> 32));
+        for (int i = 0; i < len; ++i) {
+            const uint32_t r = mix(key + (uint32_t)i * 0x9E3779B1u);
+            sm[e0 + i] = code_of(m[i], em[b], 1, (r & 0xFFFFu) / 65536.0);
+            sv[e0 + i] = code_of(v[i], ev[b], 0, (r >> 16) / 65536.0);
+        }
+    }
+    orc_cast(d->master, d->grad_param, d->dtype, d->n_shard);
+}
+
+int elx_adam8_multi(const ElxChunkDesc* descs, int first, int count, int64_t n_tiles, int dtype, const ElxSeg* segs,
+                    const ElxHyper* hyper, int n_groups, ElxCtl* ctl, void* stream) {
+    (void)n_tiles;
+    (void)stream;
+    if (!descs || !ctl) return ELX_ERR_NULL;
+    if (n_groups > 64) return ELX_ERR_CAPACITY;
+    for (int c = first; c < first + count; ++c) {
+        if (descs[c].dtype != dtype) {
+            ctl->status |= ELX_STAT_BAD_DESC;
+            continue;
+        }
+        adam8_shard(&descs[c], c, segs, hyper, n_groups, ctl);
+    }
+    return ELX_OK;
+}
+
+int elx_moments_pack(const float* exp_avg, const float* exp_avg_sq, int64_t n, void* state_m, void* state_v, void* stream) {
+    (void)stream;
+    if (!exp_avg || !exp_avg_sq || !state_m || !state_v) return ELX_ERR_NULL;
+    if (n < 0) return ELX_ERR_SIZE;
+    for (int k = 0; k < 2; ++k) {
+        const float* x = k ? exp_avg_sq : exp_avg;
+        uint8_t* s = (uint8_t*)(k ? state_v : state_m);
+        for (int64_t b = 0; b < blocks_of(n); ++b) {
+            const int64_t e0 = b * ELX_MOMENT_BLOCK;
+            const int len = (int)(n - e0 < ELX_MOMENT_BLOCK ? n - e0 : ELX_MOMENT_BLOCK);
+            const uint8_t e = block_exp(x + e0, len);
+            s[exps_at(n) + b] = e;
+            for (int i = 0; i < len; ++i) s[e0 + i] = code_of(x[e0 + i], e, !k, 0.5);
+        }
+    }
+    return ELX_OK;
+}
+
+int elx_moments_unpack(const void* state_m, const void* state_v, int64_t n, int dtype, void* exp_avg, void* exp_avg_sq,
+                       void* stream) {
+    (void)stream;
+    if (!state_m || !state_v || !exp_avg || !exp_avg_sq) return ELX_ERR_NULL;
+    if (dtype != ELX_F32 && dtype != ELX_BF16) return ELX_ERR_DTYPE;
+    if (n < 0) return ELX_ERR_SIZE;
+    for (int k = 0; k < 2; ++k) {
+        const uint8_t* s = (const uint8_t*)(k ? state_v : state_m);
+        void* out = k ? exp_avg_sq : exp_avg;
+        for (int64_t i = 0; i < n; ++i) {
+            const float x = code_value(s[i], s[exps_at(n) + i / ELX_MOMENT_BLOCK], !k);
+            if (dtype == ELX_F32) ((float*)out)[i] = x;
+            else orc_cast(&x, (uint16_t*)out + i, ELX_BF16, 1);
+        }
+    }
+    return ELX_OK;
+}
+
+/* The operators of the wrapped model have no host-memory form: CPU tensors stay with torch. */
+int elx_layer_norm_forward(const void* x, const void* weight, const void* bias, int dtype, int64_t rows, int64_t cols,
+                           float eps, void* y, float* mean, float* rstd, void* stream) {
+    (void)x; (void)weight; (void)bias; (void)dtype; (void)rows; (void)cols; (void)eps; (void)y; (void)mean; (void)rstd;
+    (void)stream;
+    return ELX_ERR_NODEVICE;
+}
+int64_t elx_layer_norm_backward_workspace(int64_t rows, int64_t cols) {
+    (void)rows; (void)cols;
+    return ELX_ERR_NODEVICE;
+}
+int elx_layer_norm_backward(const void* dy, const void* x, const void* weight, const float* mean, const float* rstd, int dtype,
+                            int64_t rows, int64_t cols, void* dx, void* dweight, void* dbias, void* workspace,
+                            int64_t workspace_bytes, void* stream) {
+    (void)dy; (void)x; (void)weight; (void)mean; (void)rstd; (void)dtype; (void)rows; (void)cols; (void)dx; (void)dweight;
+    (void)dbias; (void)workspace; (void)workspace_bytes; (void)stream;
+    return ELX_ERR_NODEVICE;
+}
+int elx_embedding_forward(const void* tokens, int index_bytes, int64_t n, const void* weight, int dtype, int64_t vocab,
+                          int64_t width, float scale, void* out, void* stream) {
+    (void)tokens; (void)index_bytes; (void)n; (void)weight; (void)dtype; (void)vocab; (void)width; (void)scale; (void)out;
+    (void)stream;
+    return ELX_ERR_NODEVICE;
+}
+int64_t elx_embedding_backward_workspace(int64_t n, int64_t width) {
+    (void)n; (void)width;
+    return ELX_ERR_NODEVICE;
+}
+int elx_embedding_backward(const void* tokens, int index_bytes, int64_t n, const void* dout, int dtype, int64_t vocab,
+                           int64_t width, float scale, int64_t padding_idx, void* dweight, void* workspace,
+                           int64_t workspace_bytes, void* stream) {
+    (void)tokens; (void)index_bytes; (void)n; (void)dout; (void)dtype; (void)vocab; (void)width; (void)scale;
+    (void)padding_idx; (void)dweight; (void)workspace; (void)workspace_bytes; (void)stream;
+    return ELX_ERR_NODEVICE;
 }
