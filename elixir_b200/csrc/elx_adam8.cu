@@ -8,29 +8,168 @@ using namespace elx;
 
 namespace {
 
-__device__ __forceinline__ float sqrt_approx(float x) {
+// ------------------------------------------------------------------------------------------------
+// one element
+// ------------------------------------------------------------------------------------------------
+
+// What the update needs of a parameter group beside GroupK, with powers of two folded in: the second moment is scaled
+// by 2^24 before its root, so that its smallest subnormal is a normal number there and the flushing forms of root and
+// reciprocal (one instruction each) lose nothing; 2^12 then stands in eps and in the first moment's factor as well.
+struct Group8 {
+    float lr, beta1, omb1, beta2, omb2, wd_l2, wd_w;
+    float rbc1, rbc2, eps;   // 2^12 / bc1, 2^24 / bc2, 2^12 eps
+};
+
+__device__ __forceinline__ Group8 pack_group8(const GroupK& k) {
+    Group8 g;
+    g.lr = k.lr;
+    g.beta1 = k.beta1;
+    g.omb1 = k.omb1;
+    g.beta2 = k.beta2;
+    g.omb2 = k.omb2;
+    g.wd_l2 = k.wd_l2;
+    g.wd_w = k.wd_w;
+    g.rbc1 = k.rbc1 * 4096.0f;
+    g.rbc2 = k.rbc2 * 16777216.0f;
+    g.eps = k.eps * 4096.0f;
+    return g;
+}
+
+__device__ __forceinline__ float unscale(float g, int div_mode, float div, float inv_div) {
+    if (div_mode == kMulInv) return g * inv_div;   // exact: the divisor is a power of two
+    return div_mode == kTrueDiv ? div_or_zero(g, div) : g;
+}
+
+// The new moments: fp32 numbers with every product and sum rounded once, no fused multiply-add.  Which code they get
+// hangs on their last bit, and so it is the same wherever the operation is restated.
+__device__ __forceinline__ void new_moments(float p, float& m, float& v, float g, const Group8& k) {
+    if (k.wd_l2 != 0.0f) g = fmaf(k.wd_l2, p, g);   // uniform: one group per call site's block, or the element-wise path
+    m = __fadd_rn(__fmul_rn(k.beta1, m), __fmul_rn(k.omb1, g));
+    v = __fadd_rn(__fmul_rn(k.beta2, v), __fmul_rn(__fmul_rn(k.omb2, g), g));
+}
+
+// The parameter's step, by the unrounded (fp32) moments: approximate root and reciprocal, off by a few 2^-23 in a term
+// that is lr times smaller than what the parameter's own rounding allows to be seen.  For second moments below 2^31.
+__device__ __forceinline__ float new_param(float p, float m, float v, const Group8& k) {
+    float root, inv;
+    asm("sqrt.approx.ftz.f32 %0, %1;" : "=f"(root) : "f"(v * k.rbc2));
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(inv) : "f"(root + k.eps));
+    return fmaf(-k.lr, fmaf(k.wd_w, p, m * k.rbc1 * inv), p);
+}
+// The same for moments of any size.
+__device__ __noinline__ float new_param_wide(float p, float m, float v, const Group8& k) {
+    const float root = sqrtf(v * (k.rbc2 * 0x1p-24f)) * 4096.0f;
+    return fmaf(-k.lr, fmaf(k.wd_w, p, m * k.rbc1 / (root + k.eps)), p);
+}
+
+// Exponent bytes up to which one product decodes or encodes (2^(E - 15), 2^(15 - E) and, for the second moment,
+// 2^(E - 31), 2^(31 - E) are normal numbers): first moments below 2^15, second moments below 2^31.  Others, and blocks
+// that are not finite, take the element-wise path.
+constexpr uint32_t kEasyM = 141, kEasyV = 157;
+
+// ------------------------------------------------------------------------------------------------
+// one block of 256 elements by one warp, element by element
+// ------------------------------------------------------------------------------------------------
+
+struct BlockAt {
+    float* p;              // first element of the block in each array: shared or global memory
+    const void* g;
+    void* lowp;            // may be g itself
+    uint8_t *cm, *cv;
+    uint8_t *em, *ev;
+    int64_t e0;            // its index in the shard
+    int len;
+    const ElxSeg* segs;
+    int n_segs;
+    int group;             // group of the whole block, or -1: look each element up
+};
+
+// Shard tail, segment boundary, uncovered elements, unaligned arrays, moments of extreme size.  An uncovered element of
+// a block that is updated keeps the values of its moments, under the block's new scale.
+template <int DT>
+__device__ __noinline__ void update_block(const BlockAt& b, const Group8* s_group, int n_groups, uint32_t key, int div_mode,
+                                          float div, float inv_div, float& nan_acc) {
+    using T = typename Lp<DT>::T;
+    const int lane = threadIdx.x & 31;
+    const uint32_t em0 = *b.em, ev0 = *b.ev;
+    const float sm = decode_scale(em0), sv = decode_scale(ev0);
+    float m[8], v[8], p[8];
+    int grp[8];
+    uint32_t top_m = 0, top_v = 0;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+        const int i = lane + 32 * j;
+        m[j] = v[j] = p[j] = 0.0f;
+        grp[j] = -1;
+        if (i >= b.len) continue;
+        p[j] = b.p[i];
+        m[j] = decode<FirstMoment>(b.cm[i], sm);
+        v[j] = decode<SecondMoment>(b.cv[i], sv);
+        grp[j] = b.group;
+        if (b.group < 0) {
+            const int si = find_seg(b.segs, b.n_segs, b.e0 + i);
+            if (si >= 0 && b.e0 + i < b.segs[si].end) grp[j] = b.segs[si].group;
+        }
+        if (grp[j] >= 0 && grp[j] < n_groups) {
+            const float g = Lp<DT>::to_float(static_cast<const T*>(b.g)[i]);
+            nan_acc = fmaf(0.0f, g, nan_acc);
+            new_moments(p[j], m[j], v[j], unscale(g, div_mode, div, inv_div), s_group[grp[j]]);
+        } else {
+            grp[j] = -1;
+        }
+        top_m = max(top_m, __float_as_uint(m[j]) & 0x7FFFFFFFu);
+        top_v = max(top_v, __float_as_uint(v[j]) & 0x7FFFFFFFu);
+    }
+    const uint32_t em = block_exponent(__reduce_max_sync(0xFFFFFFFFu, top_m));
+    const uint32_t ev = block_exponent(__reduce_max_sync(0xFFFFFFFFu, top_v));
+    const float xm = encode_scale(em), xv = encode_scale(ev);
+    const bool easy = em <= kEasyM && ev <= kEasyV;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+        const int i = lane + 32 * j;
+        if (i >= b.len) continue;
+        const uint32_t r = dither_bits(key, i);
+        b.cm[i] = static_cast<uint8_t>(encode<FirstMoment>(m[j], xm, (r & 0xFFFFu) << 4));
+        b.cv[i] = static_cast<uint8_t>(encode<SecondMoment>(v[j], xv, (r >> 16) << 4));
+        if (grp[j] >= 0) {
+            const Group8& k = s_group[grp[j]];
+            p[j] = easy ? new_param(p[j], m[j], v[j], k) : new_param_wide(p[j], m[j], v[j], k);
+            b.p[i] = p[j];
+        }
+        static_cast<T*>(b.lowp)[i] = Lp<DT>::from_float(p[j]);
+    }
+    if (lane == 0) {
+        *b.em = static_cast<uint8_t>(em);
+        *b.ev = static_cast<uint8_t>(ev);
+    }
+}
+
+// Byte j of a word moved to the top of a word, and the top bytes of four words as one word.
+__device__ __forceinline__ uint32_t byte_to_top(uint32_t w, int j) { return __byte_perm(w, 0, 0x0444 | (j << 12)); }
+__device__ __forceinline__ uint32_t top_bytes(uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+    return __byte_perm(__byte_perm(a, b, 0x0073), __byte_perm(c, d, 0x0073), 0x5410);
+}
+__device__ __forceinline__ float max_nan(float a, float b) {
     float r;
-    asm("sqrt.approx.f32 %0, %1;" : "=f"(r) : "f"(x));
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
     return r;
 }
 
-// One element of the update.  The new moments are fp32 numbers with every product and sum rounded once (no fused
-// multiply-add): their codes hang on the last bit, and so they are the same wherever the operation is restated.  The
-// parameter's own step uses the unrounded (fp32) moments and approximate root and division: two relative errors of a
-// few 2^-23 in a term that is lr times smaller than the parameter's own rounding allows to be seen.
-__device__ __forceinline__ void adam8_elem(float& p, float& m, float& v, float g, const GroupK& k, int div_mode,
-                                           float div, float inv_div) {
-    if (div_mode == kMulInv) g *= inv_div;   // exact: the divisor is a power of two
-    else if (div_mode == kTrueDiv) g = div_or_zero(g, div);
-    g = fmaf(k.wd_l2, p, g);
-    m = __fadd_rn(__fmul_rn(k.beta1, m), __fmul_rn(k.omb1, g));
-    v = __fadd_rn(__fmul_rn(k.beta2, v), __fmul_rn(__fmul_rn(k.omb2, g), g));
-    const float denom = sqrt_approx(v * k.rbc2) + k.eps;
-    float upd = __fdividef(m * k.rbc1, denom);
-    upd = fmaf(k.wd_w, p, upd);
-    p = fmaf(-k.lr, upd, p);
-}
-
+// ------------------------------------------------------------------------------------------------
+// the kernel
+// ------------------------------------------------------------------------------------------------
+//
+// Tiles of 4096 elements stream through a ring of stages in shared memory (cp.async.bulk in, cp.async.bulk out,
+// completion by mbarriers), as in the fp32 form of the update: one CTA per SM, 16 computing warps and one warp whose
+// first lane moves the data.  A stage is 32 KB with 16-bit gradients (8 g, 16 p, 4 + 4 codes) plus the 16 + 16 exponent
+// bytes of its 16 blocks, so six stages fit.  A warp owns one block of 256 elements of every tile: the block's exponent
+// needs the largest of its new moments, which stay in registers, and one redux instruction per moment gives it.  So no
+// computing warp ever waits for another; each tells the mover by itself that its part of the stage is done.
+//
+// The bytes bound it (16 per element of 16-bit chunks): the arithmetic is held to about 50 instructions per element,
+// of which the issue slots allow 88 at the full HBM rate -- dither bits 9, decoding and encoding 16, Adam 20 -- by
+// folding every scale into one product, keeping codes in the top byte of a word, and leaving all that is rare (huge or
+// non-finite moments, block borders) to update_block().
 struct Adam8Args {
     const ElxChunkDesc* descs;
     const ElxSeg* segs;
@@ -40,177 +179,372 @@ struct Adam8Args {
     int64_t n_tiles;
 };
 
-constexpr int kAdam8Threads = 512;                     // one warp per block of a tile
-static_assert(kAdam8Threads / 32 * kMomentBlock == kTile, "a tile is one block per warp");
+constexpr int kWarps = kTile / kMomentBlock;   // 16 computing warps, a block of the tile each
+constexpr int kComputing = 32 * kWarps;
+constexpr int kThreads = kComputing + 32;
 
-// A tile is 16 blocks of 256 elements, one per warp; a lane owns 8 consecutive elements.  The block's exponent needs
-// the largest magnitude of its new moments, which one redux instruction over the warp gives.
 template <int DT>
-__global__ void __launch_bounds__(kAdam8Threads, 2) adam8_kernel(const Adam8Args a) {
-    using T = typename Lp<DT>::T;
-    __shared__ GroupK s_group[kMaxGroups];
-    __shared__ ChunkCursor s_cur;
-    __shared__ SegCursor s_seg;
-    ElxCtl* ctl = a.ctl;
-    const bool skip = ctl->skip != 0;
-    const float div = ctl->div_scale, inv_div = ctl->inv_div;
-    const int div_mode = div > 0.0f ? (inv_div != 0.0f ? kMulInv : kTrueDiv) : kNoDiv;
-    const int step = ctl->step;
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    if (!skip)
-        for (int gi = threadIdx.x; gi < a.n_groups; gi += blockDim.x) s_group[gi] = derive_group(a.hyper[gi], step);
-    if (threadIdx.x == 0) {
-        s_seg.b = s_seg.e = 0;
-        s_seg.group = -1;
-        s_seg.chunk = -1;
+struct Stage8 {
+    static constexpr int kP = 0;
+    static constexpr int kG = 4 * kTile;
+    static constexpr int kGBytes = kTile * Lp<DT>::kBytes;
+    static constexpr int kM = kG + kGBytes;
+    static constexpr int kV = kM + kTile;
+    static constexpr int kEm = kV + kTile;
+    static constexpr int kEv = kEm + kWarps;
+    static constexpr int kLoaded = kEv + kWarps;
+    static constexpr int kBytes = (kLoaded + 127) / 128 * 128;
+    static constexpr int kStages = DT == ELX_F32 ? 5 : 6;
+};
+
+// kRefresh: a whole tile that gets only its working copy (no segment covers it, or the step is skipped).
+enum { kBad = 0, kWhole = 1, kRefresh = 2, kRagged = 3 };
+
+struct Slot8 {
+    float* master;
+    void* lowp;
+    const void* gsrc;
+    uint8_t *state_m, *state_v, *exps_m, *exps_v;
+    const ElxSeg* segs;
+    int64_t e0, e1, n_valid;
+    int n_segs, group, kind, chunk;
+};
+
+// The mover's view of the table: the descriptor and the segment it is in.
+struct Cursor8 {
+    int64_t t0 = 0, t1 = 0;
+    int index = -1;
+    bool vec_ok = false;
+    ElxChunkDesc d;
+    int64_t seg_b = 0, seg_e = 0;
+    int seg_group = -1;
+};
+
+template <int DT>
+__device__ __forceinline__ void classify(const Adam8Args& a, int64_t t, bool skip, Cursor8& c, Slot8& out) {
+    if (!(t >= c.t0 && t < c.t1)) {
+        int lo = a.first, hi = a.first + a.count - 1;
+        while (lo < hi) {
+            const int mid = (lo + hi + 1) >> 1;
+            if (a.descs[mid].tile_begin <= t) lo = mid; else hi = mid - 1;
+        }
+        c.d = a.descs[lo];
+        c.index = lo;
+        c.t0 = c.d.tile_begin;
+        c.t1 = c.t0 + tiles_of(c.d.n_shard);
+        c.seg_b = c.seg_e = 0;
+        const uintptr_t bits = reinterpret_cast<uintptr_t>(c.d.master) | reinterpret_cast<uintptr_t>(c.d.exp_avg) |
+                               reinterpret_cast<uintptr_t>(c.d.exp_avg_sq) | reinterpret_cast<uintptr_t>(c.d.grad_param) |
+                               reinterpret_cast<uintptr_t>(c.d.grad_src);
+        c.vec_ok = (bits & 15u) == 0;
     }
-    cursor_reset(s_cur);
+    if (!(t >= c.t0 && t < c.t1) || c.d.dtype != DT) {
+        out.kind = kBad;
+        return;
+    }
+    out.e0 = (t - c.t0) * kTile;
+    out.e1 = min(out.e0 + kTile, c.d.n_shard);
+    out.segs = a.segs + c.d.seg_first;
+    out.n_segs = c.d.seg_count;
+    if (out.e0 < c.seg_b || out.e0 >= c.seg_e) {
+        const int si = find_seg(out.segs, out.n_segs, out.e0);
+        c.seg_b = si >= 0 ? out.segs[si].begin : 0;
+        c.seg_e = si >= 0 ? out.segs[si].end : 0;
+        c.seg_group = si >= 0 ? out.segs[si].group : -1;
+    }
+    const bool one = c.seg_b <= out.e0 && out.e1 <= c.seg_e && c.seg_group >= 0 && c.seg_group < a.n_groups;
+    out.group = one ? c.seg_group : -1;
+    out.master = c.d.master;
+    out.lowp = c.d.grad_param;
+    out.gsrc = grad_source(c.d);
+    out.state_m = reinterpret_cast<uint8_t*>(c.d.exp_avg);
+    out.state_v = reinterpret_cast<uint8_t*>(c.d.exp_avg_sq);
+    out.exps_m = out.state_m + moment_exps_at(c.d.n_shard);
+    out.exps_v = out.state_v + moment_exps_at(c.d.n_shard);
+    out.n_valid = c.d.n_valid;
+    out.chunk = c.index;
+    const bool whole = out.e1 - out.e0 == kTile && c.vec_ok;
+    if (whole && (skip || (!one && range_uncovered(out.segs, out.n_segs, out.e0, out.e1, c.d.n_valid)))) out.kind = kRefresh;
+    else out.kind = whole && one ? kWhole : kRagged;
+}
+
+template <int DT>
+__global__ void __launch_bounds__(kThreads, 1) adam8_kernel(const __grid_constant__ Adam8Args a) {
+    using S = Stage8<DT>;
+    using T = typename Lp<DT>::T;
+    constexpr int kStages = S::kStages;
+    extern __shared__ __align__(128) unsigned char s_dyn[];
+    __shared__ Group8 s_group[kMaxGroups];
+    __shared__ Slot8 s_slot[kStages];
+    __shared__ __align__(8) uint64_t s_full[kStages];   // the loads of a stage have landed (and its slot is published)
+    __shared__ __align__(8) uint64_t s_done[kStages];   // all computing warps are through with a stage
+    __shared__ int s_abort;
+    static_assert(kStages * S::kBytes + sizeof(s_group) + sizeof(s_slot) + 2 * sizeof(s_full) + 64 <= 227 * 1024, "shared memory");
+
+    ElxCtl* const ctl = a.ctl;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const bool skip = ctl->skip != 0;
+    const int step = ctl->step;
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < kStages; ++s) {
+            mbar_init(&s_full[s], 1);
+            mbar_init(&s_done[s], kWarps);
+        }
+        s_abort = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    __syncthreads();
 
     const int64_t tile_lo = a.descs[a.first].tile_begin;
+    const int64_t my_tiles = blockIdx.x < a.n_tiles ? (a.n_tiles - blockIdx.x + gridDim.x - 1) / gridDim.x : 0;
+
+    if (warp == kWarps) {
+        if (lane == 0) {
+            Cursor8 cur;
+            auto produce = [&](int64_t k) {
+                const int s = static_cast<int>(k % kStages);
+                unsigned char* const at = s_dyn + s * S::kBytes;
+                Slot8 slot;
+                classify<DT>(a, tile_lo + blockIdx.x + k * gridDim.x, skip, cur, slot);
+                s_slot[s] = slot;
+                if (slot.kind == kWhole) {
+                    const int64_t block = slot.e0 / kMomentBlock;
+                    mbar_arrive_expect_tx(&s_full[s], S::kLoaded);
+                    bulk_g2s(at + S::kP, slot.master + slot.e0, 4 * kTile, &s_full[s]);
+                    bulk_g2s(at + S::kG, static_cast<const T*>(slot.gsrc) + slot.e0, S::kGBytes, &s_full[s]);
+                    bulk_g2s(at + S::kM, slot.state_m + slot.e0, kTile, &s_full[s]);
+                    bulk_g2s(at + S::kV, slot.state_v + slot.e0, kTile, &s_full[s]);
+                    bulk_g2s(at + S::kEm, slot.exps_m + block, kWarps, &s_full[s]);
+                    bulk_g2s(at + S::kEv, slot.exps_v + block, kWarps, &s_full[s]);
+                } else if (slot.kind == kRefresh) {
+                    mbar_arrive_expect_tx(&s_full[s], 4 * kTile);
+                    bulk_g2s(at + S::kP, slot.master + slot.e0, 4 * kTile, &s_full[s]);
+                } else {
+                    mbar_arrive(&s_full[s]);   // nothing to load: publishes the slot
+                }
+            };
+            for (int64_t k = 0; k < my_tiles && k < kStages - 1; ++k) produce(k);
+            int64_t k = 0;
+            for (; k < my_tiles; ++k) {
+                const int s = static_cast<int>(k % kStages);
+                const uint32_t parity = static_cast<uint32_t>((k / kStages) & 1);
+                bool handed_over = false;
+                for (uint32_t i = 0; i < kTmaSpinLimit && !handed_over; ++i) {
+                    handed_over = mbar_try_wait(&s_done[s], parity);
+                    if (!handed_over && *reinterpret_cast<volatile int*>(&s_abort)) break;
+                }
+                if (!handed_over) {
+                    s_abort = 1;
+                    break;
+                }
+                const Slot8 slot = s_slot[s];
+                unsigned char* const at = s_dyn + s * S::kBytes;
+                if (slot.kind == kWhole || slot.kind == kRefresh)
+                    bulk_s2g(static_cast<T*>(slot.lowp) + slot.e0, at + S::kG, S::kGBytes);
+                if (slot.kind == kWhole) {
+                    const int64_t block = slot.e0 / kMomentBlock;
+                    bulk_s2g(slot.master + slot.e0, at + S::kP, 4 * kTile);
+                    bulk_s2g(slot.state_m + slot.e0, at + S::kM, kTile);
+                    bulk_s2g(slot.state_v + slot.e0, at + S::kV, kTile);
+                    bulk_s2g(slot.exps_m + block, at + S::kEm, kWarps);
+                    bulk_s2g(slot.exps_v + block, at + S::kEv, kWarps);
+                }
+                bulk_commit();
+                if (k + kStages - 1 < my_tiles) {
+                    bulk_wait_read<1>();   // the stage of tile k-1 has been read out by its stores
+                    produce(k + kStages - 1);
+                }
+            }
+            if (s_abort) {
+                // the loads already issued still target this CTA's shared memory: wait (bounded again) for them
+                for (int64_t j = k; j < my_tiles && j < k + kStages - 1; ++j)
+                    (void)mbar_wait_bounded(&s_full[j % kStages], static_cast<uint32_t>((j / kStages) & 1));
+                atomicOr(&ctl->status, ELX_STAT_TIMEOUT);
+            }
+            bulk_wait_all();
+        }
+        return;
+    }
+
+    // the computing warps; the group constants take shape while the first tiles are on their way
+    const float div = ctl->div_scale, inv_div = ctl->inv_div;
+    const int div_mode = div > 0.0f ? (inv_div != 0.0f ? kMulInv : kTrueDiv) : kNoDiv;
+    if (!skip)
+        for (int gi = threadIdx.x; gi < a.n_groups; gi += kComputing) s_group[gi] = pack_group8(derive_group(a.hyper[gi], step));
+    asm volatile("bar.sync 1, %0;" ::"n"(kComputing) : "memory");
+
     float nan_acc = 0.0f;
     bool bad_desc = false;
-    for (int64_t it = blockIdx.x; it < a.n_tiles; it += gridDim.x) {
-        const int64_t t = tile_lo + it;
-        if (!locate_chunk(a.descs, a.first, a.count, t, s_cur) || s_cur.d.dtype != DT) {
-            bad_desc = true;
-            continue;
+    Group8 k8 = {};
+    int have = -1;
+    for (int64_t k = 0; k < my_tiles; ++k) {
+        const int s = static_cast<int>(k % kStages);
+        if (!mbar_wait_bounded(&s_full[s], static_cast<uint32_t>((k / kStages) & 1)) || *reinterpret_cast<volatile int*>(&s_abort)) {
+            s_abort = 1;
+            break;
         }
-        const int64_t n = s_cur.d.n_shard;
-        const int64_t e0 = (t - s_cur.t0) * kTile;
-        const int64_t e1 = min(e0 + kTile, n);
-        const ElxSeg* csegs = a.segs + s_cur.d.seg_first;
-        const int n_segs = s_cur.d.seg_count;
-        if (s_seg.chunk != s_cur.index || e0 < s_seg.b || e0 >= s_seg.e) {
-            __syncthreads();
-            if (threadIdx.x == 0) {
-                const int si = find_seg(csegs, n_segs, e0);
-                s_seg.chunk = s_cur.index;
-                s_seg.b = si >= 0 ? csegs[si].begin : 0;
-                s_seg.e = si >= 0 ? csegs[si].end : 0;
-                s_seg.group = si >= 0 ? csegs[si].group : -1;
-            }
-            __syncthreads();
-        }
-        const int grp = s_seg.group;
-        const bool one_group = s_seg.b <= e0 && e1 <= s_seg.e && grp >= 0 && grp < a.n_groups;
-        float* const master = s_cur.d.master;
-        T* const lowp = static_cast<T*>(s_cur.d.grad_param);
-        const T* const gsrc = static_cast<const T*>(grad_source(s_cur.d));
-        uint8_t* const state_m = reinterpret_cast<uint8_t*>(s_cur.d.exp_avg);
-        uint8_t* const state_v = reinterpret_cast<uint8_t*>(s_cur.d.exp_avg_sq);
-        uint8_t* const exps_m = state_m + moment_exps_at(n);
-        uint8_t* const exps_v = state_v + moment_exps_at(n);
-        const int64_t b0 = e0 + warp * kMomentBlock;   // first element of the warp's block
-        if (b0 >= e1) continue;
-        const int64_t block = b0 / kMomentBlock;
+        const Slot8& slot = s_slot[s];
+        unsigned char* const at = s_dyn + s * S::kBytes;
+        float* const sp = reinterpret_cast<float*>(at + S::kP) + warp * kMomentBlock;
+        T* const sg = reinterpret_cast<T*>(at + S::kG) + warp * kMomentBlock;
+        uint8_t *const scm = at + S::kM + warp * kMomentBlock, *const scv = at + S::kV + warp * kMomentBlock;
 
-        if (!skip && e1 - e0 == kTile && s_cur.vec_ok && one_group) {
-            const GroupK k = s_group[grp];
-            const int64_t e = b0 + lane * 8;
-            float g[8], p[8];
-            load_lowp<DT, 8>(gsrc, e0, g);
-            load_f32<8>(master, e0, p);
-            const uint2 cm = *reinterpret_cast<const uint2*>(state_m + e), cv = *reinterpret_cast<const uint2*>(state_v + e);
-            const float sm = decode_scale(exps_m[block]), sv = decode_scale(exps_v[block]);
-            float m[8], v[8];
-            uint32_t top_m = 0, top_v = 0;
-#pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                m[j] = decode<FirstMoment>(((j < 4 ? cm.x : cm.y) >> (8 * (j & 3))) & 0xFFu, sm);
-                v[j] = decode<SecondMoment>(((j < 4 ? cv.x : cv.y) >> (8 * (j & 3))) & 0xFFu, sv);
-                nan_acc = fmaf(0.0f, g[j], nan_acc);
-                adam8_elem(p[j], m[j], v[j], g[j], k, div_mode, div, inv_div);
-                top_m = max(top_m, __float_as_uint(m[j]) & 0x7FFFFFFFu);
-                top_v = max(top_v, __float_as_uint(v[j]) & 0x7FFFFFFFu);
+        if (slot.kind == kWhole) {
+            if (slot.group != have) {
+                have = slot.group;
+                k8 = s_group[have];
             }
-            const uint32_t em = block_exponent(__reduce_max_sync(0xFFFFFFFFu, top_m));
-            const uint32_t ev = block_exponent(__reduce_max_sync(0xFFFFFFFFu, top_v));
-            const float xm = encode_scale(em), xv = encode_scale(ev);
-            const uint32_t key = dither_key(step, s_cur.index, block);
-            uint2 om = make_uint2(0, 0), ov = make_uint2(0, 0);
+            const int64_t block = slot.e0 / kMomentBlock + warp;
+            const uint32_t key = dither_key(step, slot.chunk, block);
+            const uint32_t em0 = at[S::kEm + warp], ev0 = at[S::kEv + warp];
+            // a lane owns 2 x 4 consecutive elements, 128 apart: conflict-free accesses of whole words
+            float p[8], m[8], v[8];
+            const float dm = em0 ? __uint_as_float((em0 + 112u) << 23) : 0.0f;   // 2^(E - 15)
+            const float dv = ev0 ? __uint_as_float((ev0 + 96u) << 23) : 0.0f;    // 2^(E - 31)
+            float top_m = 0.0f, top_v = 0.0f;
 #pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                const uint32_t r = dither_bits(key, lane * 8 + j);
-                const uint32_t a0 = encode<FirstMoment>(m[j], xm, (r & 0xFFFFu) << 4) << (8 * (j & 3));
-                const uint32_t a1 = encode<SecondMoment>(v[j], xv, (r >> 16) << 4) << (8 * (j & 3));
-                if (j < 4) { om.x |= a0; ov.x |= a1; } else { om.y |= a0; ov.y |= a1; }
-            }
-            store_f32<8>(master, e0, p);
-            store_lowp<DT, 8>(lowp, e0, p);
-            *reinterpret_cast<uint2*>(state_m + e) = om;
-            *reinterpret_cast<uint2*>(state_v + e) = ov;
-            if (lane == 0) {
-                exps_m[block] = static_cast<uint8_t>(em);
-                exps_v[block] = static_cast<uint8_t>(ev);
-            }
-            continue;
-        }
-
-        // Skipped step, shard tail, segment boundary, uncovered elements or unaligned pointers: one element at a time.
-        // An uncovered element of a block that is updated keeps the values of its moments, under the block's new scale.
-        const int64_t b1 = min(b0 + kMomentBlock, e1);
-        const bool touched = !skip && !range_uncovered(csegs, n_segs, b0, b1, s_cur.d.n_valid);
-        float m[8], v[8];
-        uint32_t top_m = 0, top_v = 0;
-        const float sm = touched ? decode_scale(exps_m[block]) : 0.0f, sv = touched ? decode_scale(exps_v[block]) : 0.0f;
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            m[j] = v[j] = 0.0f;
-            const int64_t e = b0 + lane + 32 * j;
-            if (e >= b1) continue;
-            float p = master[e];
-            if (touched) {
-                m[j] = decode<FirstMoment>(state_m[e], sm);
-                v[j] = decode<SecondMoment>(state_v[e], sv);
-                const int si = find_seg(csegs, n_segs, e);
-                const int ge = si >= 0 && e < csegs[si].end ? csegs[si].group : -1;
-                if (ge >= 0 && ge < a.n_groups) {
-                    const float g = Lp<DT>::to_float(gsrc[e]);
-                    nan_acc = fmaf(0.0f, g, nan_acc);
-                    adam8_elem(p, m[j], v[j], g, s_group[ge], div_mode, div, inv_div);
-                    master[e] = p;
+            for (int h = 0; h < 2; ++h) {
+                const int i = h * 128 + lane * 4;
+                const float4 pp = *reinterpret_cast<const float4*>(sp + i);
+                const uint32_t cm = *reinterpret_cast<const uint32_t*>(scm + i), cv = *reinterpret_cast<const uint32_t*>(scv + i);
+                float g[4];
+                if constexpr (DT == ELX_F32) {
+                    const float4 gg = *reinterpret_cast<const float4*>(sg + i);
+                    g[0] = gg.x; g[1] = gg.y; g[2] = gg.z; g[3] = gg.w;
+                } else {
+                    const uint2 gg = *reinterpret_cast<const uint2*>(sg + i);
+                    const float2 a0 = Lp<DT>::unpack2(gg.x), a1 = Lp<DT>::unpack2(gg.y);
+                    g[0] = a0.x; g[1] = a0.y; g[2] = a1.x; g[3] = a1.y;
                 }
-                top_m = max(top_m, __float_as_uint(m[j]) & 0x7FFFFFFFu);
-                top_v = max(top_v, __float_as_uint(v[j]) & 0x7FFFFFFFu);
-            }
-            lowp[e] = Lp<DT>::from_float(p);
-        }
-        if (!touched) continue;   // the whole warp: one block, one decision
-        const uint32_t em = block_exponent(__reduce_max_sync(0xFFFFFFFFu, top_m));
-        const uint32_t ev = block_exponent(__reduce_max_sync(0xFFFFFFFFu, top_v));
-        const float xm = encode_scale(em), xv = encode_scale(ev);
-        const uint32_t key = dither_key(step, s_cur.index, block);
+                p[4 * h] = pp.x; p[4 * h + 1] = pp.y; p[4 * h + 2] = pp.z; p[4 * h + 3] = pp.w;
+                if (div_mode == kMulInv) {
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            const int64_t e = b0 + lane + 32 * j;
-            if (e >= b1) continue;
-            const uint32_t r = dither_bits(key, lane + 32 * j);
-            state_m[e] = static_cast<uint8_t>(encode<FirstMoment>(m[j], xm, (r & 0xFFFFu) << 4));
-            state_v[e] = static_cast<uint8_t>(encode<SecondMoment>(v[j], xv, (r >> 16) << 4));
+                    for (int j = 0; j < 4; ++j) g[j] *= inv_div;
+                } else if (div_mode == kTrueDiv) {
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) g[j] = div_or_zero(g[j], div);
+                }
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const int q = 4 * h + j;
+                    const uint32_t bm = byte_to_top(cm, j), bv = byte_to_top(cv, j);
+                    m[q] = __uint_as_float((static_cast<uint32_t>(static_cast<int32_t>(bm) >> 4) & 0x87F00000u)) * dm;
+                    v[q] = __uint_as_float(bv >> 4) * dv;
+                    new_moments(p[q], m[q], v[q], g[j], k8);
+                    top_m = max_nan(top_m, fabsf(m[q]));
+                    top_v = max_nan(top_v, v[q]);
+                }
+            }
+            const uint32_t em = block_exponent(__reduce_max_sync(0xFFFFFFFFu, __float_as_uint(top_m)));
+            const uint32_t ev = block_exponent(__reduce_max_sync(0xFFFFFFFFu, __float_as_uint(top_v)));
+            if (max(em, em0) <= kEasyM && max(ev, ev0) <= kEasyV) {
+                const float xm = __uint_as_float((142u - em) << 23);   // 2^(15 - E)
+                const float xv = __uint_as_float((158u - ev) << 23);   // 2^(31 - E)
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    const int i = h * 128 + lane * 4;
+                    uint32_t tm[4], tv[4];
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        const int q = 4 * h + j;
+                        const uint32_t r = dither_bits(key, i + j);
+                        // the kept bits of a code end at bit 24 after a shift by 4: the code is the top byte
+                        // (__fmul_rn and the masks are deliberate: nvcc 12.9 gets a plain product followed by byte
+                        // permutes of the dither wrong here -- all codes 0 -- and the tests of the codes show it)
+                        tm[j] = (__float_as_uint(__fmul_rn(fabsf(m[q]), xm)) << 4) + ((r & 0xFFFFu) << 8);
+                        tm[j] = (__float_as_uint(m[q]) & 0x80000000u) | tm[j];
+                        tv[j] = (__float_as_uint(__fmul_rn(v[q], xv)) << 4) + ((r >> 16) << 8);
+                        if (v[q] > 0.0f) tv[j] = max(tv[j], 0x1000000u);
+                        p[q] = new_param(p[q], m[q], v[q], k8);
+                    }
+                    *reinterpret_cast<uint32_t*>(scm + i) = top_bytes(tm[0], tm[1], tm[2], tm[3]);
+                    *reinterpret_cast<uint32_t*>(scv + i) = top_bytes(tv[0], tv[1], tv[2], tv[3]);
+                    *reinterpret_cast<float4*>(sp + i) = make_float4(p[4 * h], p[4 * h + 1], p[4 * h + 2], p[4 * h + 3]);
+                    if constexpr (DT == ELX_F32) {
+                        *reinterpret_cast<float4*>(sg + i) = make_float4(p[4 * h], p[4 * h + 1], p[4 * h + 2], p[4 * h + 3]);
+                    } else {
+                        *reinterpret_cast<uint2*>(sg + i) = make_uint2(Lp<DT>::pack2(p[4 * h], p[4 * h + 1]),
+                                                                       Lp<DT>::pack2(p[4 * h + 2], p[4 * h + 3]));
+                    }
+                }
+                __syncwarp();   // every lane has read the old exponents
+                if (lane == 0) {
+                    at[S::kEm + warp] = static_cast<uint8_t>(em);
+                    at[S::kEv + warp] = static_cast<uint8_t>(ev);
+                }
+            } else {
+                const BlockAt b = {sp, sg, sg, scm, scv, at + S::kEm + warp, at + S::kEv + warp, slot.e0 + warp * kMomentBlock,
+                                   kMomentBlock, nullptr, 0, slot.group};
+                update_block<DT>(b, s_group, a.n_groups, key, div_mode, div, inv_div, nan_acc);
+            }
+            fence_async_smem();   // the bulk stores read what the threads just wrote
+        } else if (slot.kind == kRefresh) {
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                const int i = h * 128 + lane * 4;
+                const float4 pp = *reinterpret_cast<const float4*>(sp + i);
+                if constexpr (DT == ELX_F32) *reinterpret_cast<float4*>(sg + i) = pp;
+                else *reinterpret_cast<uint2*>(sg + i) = make_uint2(Lp<DT>::pack2(pp.x, pp.y), Lp<DT>::pack2(pp.z, pp.w));
+            }
+            fence_async_smem();
+        } else if (slot.kind == kRagged) {
+            const int64_t b0 = slot.e0 + warp * kMomentBlock, b1 = min(b0 + kMomentBlock, slot.e1);
+            T* const lowp = static_cast<T*>(slot.lowp);
+            if (b0 < b1) {
+                if (!skip && (slot.group >= 0 || !range_uncovered(slot.segs, slot.n_segs, b0, b1, slot.n_valid))) {
+                    const int64_t block = b0 / kMomentBlock;
+                    int group = slot.group;
+                    if (group < 0) {   // one segment may cover the block although it does not cover the tile
+                        const int si = find_seg(slot.segs, slot.n_segs, b0);
+                        if (si >= 0 && slot.segs[si].end >= b1 && slot.segs[si].group < a.n_groups) group = slot.segs[si].group;
+                    }
+                    const BlockAt b = {slot.master + b0, static_cast<const T*>(slot.gsrc) + b0, lowp + b0, slot.state_m + b0,
+                                       slot.state_v + b0, slot.exps_m + block, slot.exps_v + block, b0, static_cast<int>(b1 - b0),
+                                       slot.segs, slot.n_segs, group};
+                    update_block<DT>(b, s_group, a.n_groups, dither_key(step, slot.chunk, block), div_mode, div, inv_div, nan_acc);
+                } else {
+                    for (int64_t e = b0 + lane; e < b1; e += 32) lowp[e] = Lp<DT>::from_float(slot.master[e]);
+                }
+            }
+        } else {
+            bad_desc = true;
         }
-        if (lane == 0) {
-            exps_m[block] = static_cast<uint8_t>(em);
-            exps_v[block] = static_cast<uint8_t>(ev);
-        }
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&s_done[s]);
     }
 
     const unsigned late = __ballot_sync(0xFFFFFFFFu, nan_acc != nan_acc);
-    const unsigned bad = __ballot_sync(0xFFFFFFFFu, bad_desc);
     if (lane == 0) {
         if (late) {
             atomicOr(&ctl->late_inf, 1u);
             atomicOr(&ctl->status, ELX_STAT_LATE_INF);
         }
-        if (bad) atomicOr(&ctl->status, ELX_STAT_BAD_DESC);
+        if (bad_desc) atomicOr(&ctl->status, ELX_STAT_BAD_DESC);
     }
 }
 
 template <int DT>
 int launch_adam8(const Adam8Args& a, cudaStream_t s) {
-    static const int resident = resident_ctas(adam8_kernel<DT>, kAdam8Threads);
-    const int grid = grid_for(a.n_tiles, resident);
+    constexpr int smem = Stage8<DT>::kStages * Stage8<DT>::kBytes;
+    // the opt-in to more than 48 KB of dynamic shared memory is per device: once for each ordinal
+    static bool opted_in[64];
+    int dev = -1;
+    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) {
+        (void)cudaGetLastError();
+        return ELX_ERR_NODEVICE;
+    }
+    if (!opted_in[dev]) {
+        const cudaError_t attr = cudaFuncSetAttribute(adam8_kernel<DT>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+        if (attr != cudaSuccess) {
+            const int rc = record_cuda(attr);
+            (void)cudaGetLastError();
+            return rc;
+        }
+        opted_in[dev] = true;
+    }
+    const int grid = grid_for(a.n_tiles, 1);
     if (grid < 0) return grid;
-    adam8_kernel<DT><<<grid, kAdam8Threads, 0, s>>>(a);
+    adam8_kernel<DT><<<grid, kThreads, smem, s>>>(a);
     return record_cuda(cudaGetLastError());
 }
 
@@ -219,94 +553,124 @@ int launch_adam8(const Adam8Args& a, cudaStream_t s) {
 // ------------------------------------------------------------------------------------------------
 
 constexpr int kConvThreads = 256;
+constexpr int kPair = 2 * kMomentBlock;   // elements a warp converts at a time: 16 lanes per block, 16 elements per lane
 
-// One warp per block and moment array; the two moments of a block one after the other.
+// One block by one warp, element by element: the end of a shard, and arrays that are not aligned.
 template <class M>
-__device__ __forceinline__ void pack_block(const float* __restrict__ x, uint8_t* state, int64_t n, int64_t block, bool vec) {
+__device__ __noinline__ void pack_block(const float* __restrict__ x, uint8_t* state, int64_t n, int64_t block) {
     const int lane = threadIdx.x & 31;
     const int64_t b0 = block * kMomentBlock;
-    const bool whole = vec && b0 + kMomentBlock <= n;
+    if (b0 >= n) return;
     float f[8];
     uint32_t top = 0;
-    if (whole) {
-        const U8 r = ld256(x + b0 + lane * 8);
 #pragma unroll
-        for (int j = 0; j < 8; ++j) f[j] = __uint_as_float(r.x[j]);
-    } else {
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            const int64_t e = b0 + lane * 8 + j;
-            f[j] = e < n ? x[e] : 0.0f;
-        }
+    for (int j = 0; j < 8; ++j) {
+        const int64_t e = b0 + lane + 32 * j;
+        f[j] = e < n ? x[e] : 0.0f;
+        top = max(top, __float_as_uint(f[j]) & 0x7FFFFFFFu);
     }
-#pragma unroll
-    for (int j = 0; j < 8; ++j) top = max(top, __float_as_uint(f[j]) & 0x7FFFFFFFu);
     const uint32_t exp = block_exponent(__reduce_max_sync(0xFFFFFFFFu, top));
     const float scale = encode_scale(exp);
-    uint32_t w[2] = {0, 0};
 #pragma unroll
-    for (int j = 0; j < 8; ++j) w[j / 4] |= encode<M>(f[j], scale, kRoundNearest) << (8 * (j & 3));
-    if (whole) {
-        *reinterpret_cast<uint2*>(state + b0 + lane * 8) = make_uint2(w[0], w[1]);
-    } else {
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            const int64_t e = b0 + lane * 8 + j;
-            if (e < n) state[e] = static_cast<uint8_t>(w[j / 4] >> (8 * (j & 3)));
-        }
+    for (int j = 0; j < 8; ++j) {
+        const int64_t e = b0 + lane + 32 * j;
+        if (e < n) state[e] = static_cast<uint8_t>(encode<M>(f[j], scale, kRoundNearest));
     }
     if (lane == 0) state[moment_exps_at(n) + block] = static_cast<uint8_t>(exp);
 }
 
+template <class M>
+__device__ __forceinline__ void pack_pair(const float* __restrict__ x, uint8_t* state, int64_t n, int64_t pair) {
+    const int lane = threadIdx.x & 31;
+    const int64_t e = pair * kPair + lane * 16;
+    float f[16];
+    uint32_t top = 0;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+        const U8 r = ld256(x + e + 8 * h);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            f[8 * h + j] = __uint_as_float(r.x[j]);
+            top = max(top, r.x[j] & 0x7FFFFFFFu);
+        }
+    }
+#pragma unroll
+    for (int o = 8; o > 0; o >>= 1) top = max(top, __shfl_xor_sync(0xFFFFFFFFu, top, o));
+    const uint32_t exp = block_exponent(top);
+    const float scale = encode_scale(exp);
+    uint32_t w[4] = {0, 0, 0, 0};
+#pragma unroll
+    for (int j = 0; j < 16; ++j) w[j / 4] |= encode<M>(f[j], scale, kRoundNearest) << (8 * (j & 3));
+    *reinterpret_cast<uint4*>(state + e) = make_uint4(w[0], w[1], w[2], w[3]);
+    if ((lane & 15) == 0) state[moment_exps_at(n) + pair * 2 + (lane >> 4)] = static_cast<uint8_t>(exp);
+}
+
+// Bound by the bytes: 8 in and 2 out per element, 7 of 8 of them in whole lines per warp.
 __global__ void __launch_bounds__(kConvThreads) pack_kernel(const float* __restrict__ m, const float* __restrict__ v, int64_t n,
                                                             uint8_t* state_m, uint8_t* state_v, int vec) {
-    const int64_t blocks = moment_blocks(n);
-    const int64_t stride = static_cast<int64_t>(gridDim.x) * (kConvThreads / 32);
-    for (int64_t b = blockIdx.x * (kConvThreads / 32) + (threadIdx.x >> 5); b < blocks; b += stride) {
-        pack_block<FirstMoment>(m, state_m, n, b, vec);
-        pack_block<SecondMoment>(v, state_v, n, b, vec);
+    const int64_t pairs = (n + kPair - 1) / kPair, stride = static_cast<int64_t>(gridDim.x) * (kConvThreads / 32);
+    for (int64_t q = blockIdx.x * (kConvThreads / 32) + (threadIdx.x >> 5); q < pairs; q += stride) {
+        if (vec && (q + 1) * kPair <= n) {
+            pack_pair<FirstMoment>(m, state_m, n, q);
+            pack_pair<SecondMoment>(v, state_v, n, q);
+        } else {
+            for (int64_t b = 2 * q; b < 2 * q + 2; ++b) {
+                pack_block<FirstMoment>(m, state_m, n, b);
+                pack_block<SecondMoment>(v, state_v, n, b);
+            }
+        }
     }
 }
 
 template <class M, int DT>
-__device__ __forceinline__ void unpack_block(const uint8_t* __restrict__ state, void* out, int64_t n, int64_t block, bool vec) {
-    using T = typename Lp<DT>::T;
-    const int lane = threadIdx.x & 31;
-    const int64_t e0 = block * kMomentBlock + lane * 8;
-    const float scale = decode_scale(state[moment_exps_at(n) + block]);
-    T* const o = static_cast<T*>(out);
-    if (vec && (block + 1) * kMomentBlock <= n) {
-        const uint2 c = *reinterpret_cast<const uint2*>(state + e0);
-        float f[8];
+__device__ __forceinline__ void unpack_codes(const uint4& c, float scale, typename Lp<DT>::T* out) {
+    const uint32_t w[4] = {c.x, c.y, c.z, c.w};
+    float f[16];
 #pragma unroll
-        for (int j = 0; j < 8; ++j) f[j] = decode<M>(((j < 4 ? c.x : c.y) >> (8 * (j & 3))) & 0xFFu, scale);
-        if constexpr (DT == ELX_F32) {
+    for (int j = 0; j < 16; ++j) f[j] = decode<M>((w[j / 4] >> (8 * (j & 3))) & 0xFFu, scale);
+    if constexpr (DT == ELX_F32) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
             U8 r;
 #pragma unroll
-            for (int j = 0; j < 8; ++j) r.x[j] = __float_as_uint(f[j]);
-            st256(o + e0, r);
-        } else {
-            U4 r;
-#pragma unroll
-            for (int j = 0; j < 4; ++j) r.x[j] = Lp<DT>::pack2(f[2 * j], f[2 * j + 1]);
-            st128(o + e0, r);
+            for (int j = 0; j < 8; ++j) r.x[j] = __float_as_uint(f[8 * h + j]);
+            st256(out + 8 * h, r);
         }
     } else {
+        U8 r;
 #pragma unroll
-        for (int j = 0; j < 8; ++j)
-            if (e0 + j < n) o[e0 + j] = Lp<DT>::from_float(decode<M>(state[e0 + j], scale));
+        for (int j = 0; j < 8; ++j) r.x[j] = Lp<DT>::pack2(f[2 * j], f[2 * j + 1]);
+        st256(out, r);
     }
 }
 
 template <int DT>
 __global__ void __launch_bounds__(kConvThreads) unpack_kernel(const uint8_t* __restrict__ state_m, const uint8_t* __restrict__ state_v,
                                                               int64_t n, void* m, void* v, int vec) {
-    const int64_t blocks = moment_blocks(n);
-    const int64_t stride = static_cast<int64_t>(gridDim.x) * (kConvThreads / 32);
-    for (int64_t b = blockIdx.x * (kConvThreads / 32) + (threadIdx.x >> 5); b < blocks; b += stride) {
-        unpack_block<FirstMoment, DT>(state_m, m, n, b, vec);
-        unpack_block<SecondMoment, DT>(state_v, v, n, b, vec);
+    using T = typename Lp<DT>::T;
+    T *const om = static_cast<T*>(m), *const ov = static_cast<T*>(v);
+    const uint8_t *const exps_m = state_m + moment_exps_at(n), *const exps_v = state_v + moment_exps_at(n);
+    const int lane = threadIdx.x & 31;
+    const int64_t pairs = (n + kPair - 1) / kPair, stride = static_cast<int64_t>(gridDim.x) * (kConvThreads / 32);
+    for (int64_t q = blockIdx.x * (kConvThreads / 32) + (threadIdx.x >> 5); q < pairs; q += stride) {
+        const int64_t e = q * kPair + lane * 16;
+        if (vec && (q + 1) * kPair <= n) {
+            const uint4 cm = __ldcs(reinterpret_cast<const uint4*>(state_m + e)), cv = __ldcs(reinterpret_cast<const uint4*>(state_v + e));
+            const float sm = decode_scale(exps_m[2 * q + (lane >> 4)]), sv = decode_scale(exps_v[2 * q + (lane >> 4)]);
+            unpack_codes<FirstMoment, DT>(cm, sm, om + e);
+            unpack_codes<SecondMoment, DT>(cv, sv, ov + e);
+        } else {
+            for (int64_t i = q * kPair + lane; i < min((q + 1) * kPair, n); i += 32) {
+                om[i] = Lp<DT>::from_float(decode<FirstMoment>(state_m[i], decode_scale(exps_m[i / kMomentBlock])));
+                ov[i] = Lp<DT>::from_float(decode<SecondMoment>(state_v[i], decode_scale(exps_v[i / kMomentBlock])));
+            }
+        }
     }
+}
+
+int conversion_grid(int64_t n) {
+    const int64_t per_block = static_cast<int64_t>(kConvThreads / 32) * kPair;
+    return grid_for((n + per_block - 1) / per_block, 8);
 }
 
 }  // namespace
@@ -339,8 +703,8 @@ int elx_moments_pack(const float* exp_avg, const float* exp_avg_sq, int64_t n, v
     if (n < 0) return ELX_ERR_SIZE;
     if (!aligned(exp_avg, 4) || !aligned(exp_avg_sq, 4)) return ELX_ERR_ALIGN;
     if (n == 0) return ELX_OK;
-    const int vec = aligned(exp_avg, 32) && aligned(exp_avg_sq, 32) && aligned(state_m, 8) && aligned(state_v, 8);
-    const int grid = grid_for((moment_blocks(n) + kConvThreads / 32 - 1) / (kConvThreads / 32), 8);
+    const int vec = aligned(exp_avg, 32) && aligned(exp_avg_sq, 32) && aligned(state_m, 16) && aligned(state_v, 16);
+    const int grid = conversion_grid(n);
     if (grid < 0) return grid;
     pack_kernel<<<grid, kConvThreads, 0, static_cast<cudaStream_t>(stream)>>>(
         exp_avg, exp_avg_sq, n, static_cast<uint8_t*>(state_m), static_cast<uint8_t*>(state_v), vec);
@@ -354,8 +718,8 @@ int elx_moments_unpack(const void* state_m, const void* state_v, int64_t n, int 
     if (n < 0) return ELX_ERR_SIZE;
     if (!aligned(exp_avg, dtype_bytes(dtype)) || !aligned(exp_avg_sq, dtype_bytes(dtype))) return ELX_ERR_ALIGN;
     if (n == 0) return ELX_OK;
-    const int vec = aligned(exp_avg, 32) && aligned(exp_avg_sq, 32) && aligned(state_m, 8) && aligned(state_v, 8);
-    const int grid = grid_for((moment_blocks(n) + kConvThreads / 32 - 1) / (kConvThreads / 32), 8);
+    const int vec = aligned(exp_avg, 32) && aligned(exp_avg_sq, 32) && aligned(state_m, 16) && aligned(state_v, 16);
+    const int grid = conversion_grid(n);
     if (grid < 0) return grid;
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     const uint8_t *sm = static_cast<const uint8_t*>(state_m), *sv = static_cast<const uint8_t*>(state_v);

@@ -48,10 +48,31 @@ def _ptr(t: Optional[torch.Tensor]):
     return None if t is None else ctypes.c_void_p(t.data_ptr())
 
 
+try:    # the handle without a Stream object around it: 0.1 us instead of 2.5 us of every call
+    from torch._C import _cuda_getCurrentRawStream as _raw_stream
+except ImportError:
+    def _raw_stream(index):
+        return torch.cuda.current_stream(index).cuda_stream
+
+
 def _stream(t: Optional[torch.Tensor]):
     if t is not None and t.is_cuda:
-        return ctypes.c_void_p(torch.cuda.current_stream(t.device).cuda_stream)
+        return ctypes.c_void_p(_raw_stream(t.get_device()))
     return None
+
+
+def _call(name: str, home: torch.Tensor, *args):
+    """Call a native entry point that ends in a stream argument, on the device of ``home`` and its current stream."""
+    entry, index = getattr(_lib.get(), name), home.get_device()
+    if index < 0:    # host-memory backend
+        status = entry(*args, None)
+    elif index == torch.cuda.current_device():
+        status = entry(*args, _raw_stream(index))
+    else:
+        with torch.cuda.device(index):
+            status = entry(*args, _raw_stream(index))
+    if status:
+        _lib.check(status, name)
 
 
 def _home(*tensors) -> Optional[torch.Tensor]:
@@ -152,10 +173,8 @@ def step_begin(ctl: ControlBlock, cfg: ElxScalerCfg, norm_sq: Optional[torch.Ten
         _check_tensor(norm_sq, 'norm_sq', torch.float32)
     if chunk_flags is not None:
         _check_tensor(chunk_flags, 'chunk_flags', torch.int32)
-    with _DeviceGuard(ctl.tensor):
-        _lib.check(_lib.get().elx_step_begin(ctl.ptr, cfg, _ptr(norm_sq), _ptr(chunk_flags),
-                                             chunk_flags.numel() if chunk_flags is not None else 0,
-                                             _stream(ctl.tensor)), 'elx_step_begin')
+    _call('elx_step_begin', ctl.tensor, ctl.tensor.data_ptr(), cfg, _addr(norm_sq), _addr(chunk_flags),
+          chunk_flags.numel() if chunk_flags is not None else 0)
 
 
 # ---------------------------------------------------------------------------------------------------
@@ -484,11 +503,8 @@ def adam_multi(table: ChunkTable, ctl: ControlBlock, first: int = 0, count: Opti
     # shards in pinned host memory are updated in place over PCIe by the load/store variant of the kernel
     name = ('elx_adam8_multi' if table.state_bits == 8 else
             'elx_adam_multi_hostmem' if table.host_resident else 'elx_adam_multi')
-    entry = getattr(_lib.get(), name)
-    with _DeviceGuard(table.descs_dev):
-        _lib.check(
-            entry(_ptr(table.descs_dev), first, count, table.tiles(first, count), table.code, _ptr(table.segs_dev),
-                  _ptr(table.hyper_dev), table.n_groups, ctl.ptr, _stream(table.descs_dev)), name)
+    _call(name, table.descs_dev, table.descs_dev.data_ptr(), first, count, table.tiles(first, count), table.code,
+          _addr(table.segs_dev), _addr(table.hyper_dev), table.n_groups, ctl.tensor.data_ptr())
 
 
 def _need_fp32_moments(*tables: ChunkTable):
@@ -678,10 +694,14 @@ def moment_state_bytes(n: int) -> int:
 
 
 def _same_device(*named):
-    home = named[0][1]
+    index = named[0][1].get_device()
     for name, t in named[1:]:
-        if t is not None and t.device != home.device:
-            raise ValueError(f'{name} is on {t.device}, {named[0][0]} on {home.device}')
+        if t is not None and t.get_device() != index:
+            raise ValueError(f'{name} is on {t.device}, {named[0][0]} on {named[0][1].device}')
+
+
+def _addr(t: Optional[torch.Tensor]):
+    return None if t is None else t.data_ptr()
 
 
 def pack_moments(exp_avg: torch.Tensor, exp_avg_sq: torch.Tensor, state_m: Optional[torch.Tensor] = None,
@@ -704,9 +724,7 @@ def pack_moments(exp_avg: torch.Tensor, exp_avg_sq: torch.Tensor, state_m: Optio
             raise ValueError(f'{name} must hold moment_state_bytes({n}) = {size} bytes')
     _same_device(('exp_avg', exp_avg), ('exp_avg_sq', exp_avg_sq), ('state_m', state_m), ('state_v', state_v))
     if n:
-        with _DeviceGuard(exp_avg):
-            _lib.check(_lib.get().elx_moments_pack(_ptr(exp_avg), _ptr(exp_avg_sq), n, _ptr(state_m), _ptr(state_v),
-                                                   _stream(exp_avg)), 'elx_moments_pack')
+        _call('elx_moments_pack', exp_avg, exp_avg.data_ptr(), exp_avg_sq.data_ptr(), n, state_m.data_ptr(), state_v.data_ptr())
     return state_m, state_v
 
 
@@ -726,9 +744,8 @@ def unpack_moments(state_m: torch.Tensor, state_v: torch.Tensor, exp_avg: torch.
             raise ValueError(f'{name} must hold moment_state_bytes({n}) = {moment_state_bytes(n)} bytes')
     _same_device(('exp_avg', exp_avg), ('exp_avg_sq', exp_avg_sq), ('state_m', state_m), ('state_v', state_v))
     if n:
-        with _DeviceGuard(exp_avg):
-            _lib.check(_lib.get().elx_moments_unpack(_ptr(state_m), _ptr(state_v), n, dtype_code(exp_avg.dtype), _ptr(exp_avg),
-                                                     _ptr(exp_avg_sq), _stream(exp_avg)), 'elx_moments_unpack')
+        _call('elx_moments_unpack', exp_avg, state_m.data_ptr(), state_v.data_ptr(), n, dtype_code(exp_avg.dtype),
+              exp_avg.data_ptr(), exp_avg_sq.data_ptr())
 
 
 # ---------------------------------------------------------------------------------------------------
@@ -758,13 +775,11 @@ def layer_norm_forward(x: torch.Tensor, weight: Optional[torch.Tensor] = None, b
     fp32, the mean and the reciprocal standard deviation that ``layer_norm_backward`` takes."""
     rows, cols = _check_norm(x, weight, bias)
     y = torch.empty_like(x)
-    stats = torch.empty((2, rows), dtype=torch.float32, device=x.device)
-    mean, rstd = stats[0], stats[1]
+    mean = torch.empty(rows, dtype=torch.float32, device=x.device)
+    rstd = torch.empty_like(mean)
     if rows:
-        with _DeviceGuard(x):
-            _lib.check(_lib.get().elx_layer_norm_forward(_ptr(x), _ptr(weight), _ptr(bias), dtype_code(x.dtype), rows, cols,
-                                                         eps, _ptr(y), _ptr(mean), _ptr(rstd), _stream(x)),
-                       'elx_layer_norm_forward')
+        _call('elx_layer_norm_forward', x, x.data_ptr(), _addr(weight), _addr(bias), dtype_code(x.dtype), rows, cols, eps,
+              y.data_ptr(), mean.data_ptr(), rstd.data_ptr())
     return y, mean, rstd
 
 
@@ -781,18 +796,15 @@ def layer_norm_backward(dy: torch.Tensor, x: torch.Tensor, weight: Optional[torc
         if t.numel() != rows:
             raise ValueError(f'{name} must have one element per row')
     _same_device(('x', x), ('dy', dy), ('mean', mean), ('rstd', rstd))
-    lib = _lib.get()
     dx = torch.empty_like(x)
     dweight = torch.empty(cols, dtype=x.dtype, device=x.device) if weight_grad and weight is not None else None
     dbias = torch.empty(cols, dtype=x.dtype, device=x.device) if bias_grad else None
     space, size = None, 0
     if dweight is not None or dbias is not None:
-        size = lib.elx_layer_norm_backward_workspace(rows, cols)
-        space = torch.empty(max(size, 16), dtype=torch.uint8, device=x.device)
-    with _DeviceGuard(x):
-        _lib.check(lib.elx_layer_norm_backward(_ptr(dy), _ptr(x), _ptr(weight), _ptr(mean), _ptr(rstd), dtype_code(x.dtype), rows,
-                                               cols, _ptr(dx), _ptr(dweight), _ptr(dbias), _ptr(space), size, _stream(x)),
-                   'elx_layer_norm_backward')
+        size = _lib.get().elx_layer_norm_backward_workspace(rows, cols)
+        space = torch.empty(size, dtype=torch.uint8, device=x.device)
+    _call('elx_layer_norm_backward', x, dy.data_ptr(), x.data_ptr(), _addr(weight), mean.data_ptr(), rstd.data_ptr(),
+          dtype_code(x.dtype), rows, cols, dx.data_ptr(), _addr(dweight), _addr(dbias), _addr(space), size)
     return dx, dweight, dbias
 
 
@@ -812,11 +824,10 @@ def embedding_forward(tokens: torch.Tensor, weight: torch.Tensor, scale: float =
     _same_device(('weight', weight), ('tokens', tokens))
     code = dtype_code(weight.dtype)
     out = torch.empty(tokens.shape + weight.shape[1:], dtype=weight.dtype, device=weight.device)
-    if tokens.numel():
-        with _DeviceGuard(weight):
-            _lib.check(_lib.get().elx_embedding_forward(_ptr(tokens), tokens.element_size(), tokens.numel(), _ptr(weight), code,
-                                                        weight.shape[0], weight.shape[1], scale, _ptr(out), _stream(weight)),
-                       'elx_embedding_forward')
+    n = tokens.numel()
+    if n:
+        _call('elx_embedding_forward', weight, tokens.data_ptr(), tokens.element_size(), n, weight.data_ptr(), code,
+              weight.shape[0], weight.shape[1], scale, out.data_ptr())
     return out
 
 
@@ -834,12 +845,9 @@ def embedding_backward(tokens: torch.Tensor, dout: torch.Tensor, vocab: int, sca
         raise ValueError('padding_idx outside the table')
     _same_device(('dout', dout), ('tokens', tokens))
     code, width, n = dtype_code(dout.dtype), dout.shape[-1], tokens.numel()
-    lib = _lib.get()
     dweight = torch.empty((vocab, width), dtype=dout.dtype, device=dout.device)
-    size = lib.elx_embedding_backward_workspace(n, width)
-    space = torch.empty(max(size, 16), dtype=torch.uint8, device=dout.device)
-    with _DeviceGuard(dout):
-        _lib.check(lib.elx_embedding_backward(_ptr(tokens), tokens.element_size(), n, _ptr(dout), code, vocab, width, scale,
-                                              -1 if padding_idx is None else padding_idx, _ptr(dweight), _ptr(space), size,
-                                              _stream(dout)), 'elx_embedding_backward')
+    size = _lib.get().elx_embedding_backward_workspace(n, width)
+    space = torch.empty(size, dtype=torch.uint8, device=dout.device)
+    _call('elx_embedding_backward', dout, tokens.data_ptr(), tokens.element_size(), n, dout.data_ptr(), code, vocab, width, scale,
+          -1 if padding_idx is None else padding_idx, dweight.data_ptr(), space.data_ptr(), size)
     return dweight
