@@ -20,19 +20,24 @@ struct Group8 {
     float rbc1, rbc2, eps;   // 2^12 / bc1, 2^24 / bc2, 2^12 eps
 };
 
-__device__ __forceinline__ Group8 pack_group8(const GroupK& k) {
-    Group8 g;
-    g.lr = k.lr;
-    g.beta1 = k.beta1;
-    g.omb1 = k.omb1;
-    g.beta2 = k.beta2;
-    g.omb2 = k.omb2;
-    g.wd_l2 = k.wd_l2;
-    g.wd_w = k.wd_w;
-    g.rbc1 = k.rbc1 * 4096.0f;
-    g.rbc2 = k.rbc2 * 16777216.0f;
-    g.eps = k.eps * 4096.0f;
-    return g;
+// By two threads per group, a moment each: the powers in double are most of a small launch's start.
+__device__ __noinline__ void derive_half(const ElxHyper& h, int step, int second, Group8& k) {
+    const float beta = second ? h.beta2 : h.beta1;
+    const double bc = h.bias_correction ? 1.0 - pow(static_cast<double>(beta), static_cast<double>(step)) : 1.0;
+    const float rbc = static_cast<float>(1.0 / bc);
+    if (second) {
+        k.beta2 = beta;
+        k.omb2 = 1.0f - beta;
+        k.rbc2 = rbc * 16777216.0f;
+        k.wd_l2 = h.adamw_mode ? 0.0f : h.weight_decay;
+        k.wd_w = h.adamw_mode ? h.weight_decay : 0.0f;
+    } else {
+        k.beta1 = beta;
+        k.omb1 = 1.0f - beta;
+        k.rbc1 = rbc * 4096.0f;
+        k.lr = h.lr;
+        k.eps = h.eps * 4096.0f;
+    }
 }
 
 __device__ __forceinline__ float unscale(float g, int div_mode, float div, float inv_div) {
@@ -80,9 +85,23 @@ struct BlockAt {
     int64_t e0;            // its index in the shard
     int len;
     const ElxSeg* segs;
-    int n_segs;
-    int group;             // group of the whole block, or -1: look each element up
+    int seg_lo, seg_hi;    // the segments that may reach into the block: [seg_lo, seg_hi]
+    int group;             // group of the whole block, or -1: by the segments
 };
+
+// The segments that reach into elements [b0, b1) of a shard, searched from segment `from` on (the last one that begins
+// at or before an earlier element, or -1).  false: none does.  group: that of a segment which covers all of them, or -1.
+__device__ __forceinline__ bool block_segments(const ElxSeg* __restrict__ segs, int n_segs, int from, int n_groups, int64_t b0, int64_t b1,
+                                               int& lo, int& hi, int& group) {
+    lo = max(from, 0);
+    group = -1;
+    while (lo < n_segs && segs[lo].end <= b0) ++lo;      // a tile's segments lie close together
+    if (lo >= n_segs || segs[lo].begin >= b1) return false;
+    hi = lo;
+    while (hi + 1 < n_segs && segs[hi + 1].begin < b1) ++hi;
+    if (segs[lo].begin <= b0 && segs[lo].end >= b1 && segs[lo].group < n_groups) group = segs[lo].group;
+    return true;
+}
 
 // Shard tail, segment boundary, uncovered elements, unaligned arrays, moments of extreme size.  An uncovered element of
 // a block that is updated keeps the values of its moments, under the block's new scale.
@@ -97,19 +116,25 @@ __device__ __noinline__ void update_block(const BlockAt& b, const Group8* s_grou
     int grp[8];
     uint32_t top_m = 0, top_v = 0;
 #pragma unroll
+    for (int j = 0; j < 8; ++j) grp[j] = b.group;
+    if (b.group < 0) {
+        for (int si = b.seg_lo; si <= b.seg_hi; ++si) {
+            const ElxSeg seg = b.segs[si];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                const int64_t e = b.e0 + lane + 32 * j;
+                if (e >= seg.begin && e < seg.end) grp[j] = seg.group;
+            }
+        }
+    }
+#pragma unroll
     for (int j = 0; j < 8; ++j) {
         const int i = lane + 32 * j;
         m[j] = v[j] = p[j] = 0.0f;
-        grp[j] = -1;
         if (i >= b.len) continue;
         p[j] = b.p[i];
         m[j] = decode<FirstMoment>(b.cm[i], sm);
         v[j] = decode<SecondMoment>(b.cv[i], sv);
-        grp[j] = b.group;
-        if (b.group < 0) {
-            const int si = find_seg(b.segs, b.n_segs, b.e0 + i);
-            if (si >= 0 && b.e0 + i < b.segs[si].end) grp[j] = b.segs[si].group;
-        }
         if (grp[j] >= 0 && grp[j] < n_groups) {
             const float g = Lp<DT>::to_float(static_cast<const T*>(b.g)[i]);
             nan_acc = fmaf(0.0f, g, nan_acc);
@@ -197,8 +222,11 @@ struct Stage8 {
     static constexpr int kStages = DT == ELX_F32 ? 5 : 6;
 };
 
-// kRefresh: a whole tile that gets only its working copy (no segment covers it, or the step is skipped).
-enum { kBad = 0, kWhole = 1, kRefresh = 2, kRagged = 3 };
+// kWhole: a whole tile inside one segment.  kMixed: a whole tile that segments cover in part or by several groups; it
+// goes through the ring all the same and each warp looks its block up.  kRefresh: a whole tile that gets only its working
+// copy (no segment reaches it, or the step is skipped).  kRagged: the end of a shard, or unaligned arrays; worked on in
+// place in global memory.
+enum { kBad = 0, kWhole = 1, kMixed = 2, kRefresh = 3, kRagged = 4 };
 
 struct Slot8 {
     float* master;
@@ -206,8 +234,8 @@ struct Slot8 {
     const void* gsrc;
     uint8_t *state_m, *state_v, *exps_m, *exps_v;
     const ElxSeg* segs;
-    int64_t e0, e1, n_valid;
-    int n_segs, group, kind, chunk;
+    int64_t e0, e1;
+    int n_segs, seg, group, kind, chunk;   // seg: the last segment that begins at or before e0, or -1
 };
 
 // The mover's view of the table: the descriptor and the segment it is in.
@@ -217,7 +245,7 @@ struct Cursor8 {
     bool vec_ok = false;
     ElxChunkDesc d;
     int64_t seg_b = 0, seg_e = 0;
-    int seg_group = -1;
+    int seg = -1, seg_group = -1;
 };
 
 template <int DT>
@@ -247,11 +275,12 @@ __device__ __forceinline__ void classify(const Adam8Args& a, int64_t t, bool ski
     out.segs = a.segs + c.d.seg_first;
     out.n_segs = c.d.seg_count;
     if (out.e0 < c.seg_b || out.e0 >= c.seg_e) {
-        const int si = find_seg(out.segs, out.n_segs, out.e0);
-        c.seg_b = si >= 0 ? out.segs[si].begin : 0;
-        c.seg_e = si >= 0 ? out.segs[si].end : 0;
-        c.seg_group = si >= 0 ? out.segs[si].group : -1;
+        c.seg = find_seg(out.segs, out.n_segs, out.e0);
+        c.seg_b = c.seg >= 0 ? out.segs[c.seg].begin : 0;
+        c.seg_e = c.seg >= 0 ? out.segs[c.seg].end : 0;
+        c.seg_group = c.seg >= 0 ? out.segs[c.seg].group : -1;
     }
+    out.seg = c.seg;
     const bool one = c.seg_b <= out.e0 && out.e1 <= c.seg_e && c.seg_group >= 0 && c.seg_group < a.n_groups;
     out.group = one ? c.seg_group : -1;
     out.master = c.d.master;
@@ -261,11 +290,12 @@ __device__ __forceinline__ void classify(const Adam8Args& a, int64_t t, bool ski
     out.state_v = reinterpret_cast<uint8_t*>(c.d.exp_avg_sq);
     out.exps_m = out.state_m + moment_exps_at(c.d.n_shard);
     out.exps_v = out.state_v + moment_exps_at(c.d.n_shard);
-    out.n_valid = c.d.n_valid;
     out.chunk = c.index;
     const bool whole = out.e1 - out.e0 == kTile && c.vec_ok;
-    if (whole && (skip || (!one && range_uncovered(out.segs, out.n_segs, out.e0, out.e1, c.d.n_valid)))) out.kind = kRefresh;
-    else out.kind = whole && one ? kWhole : kRagged;
+    if (!whole) out.kind = kRagged;
+    else if (skip) out.kind = kRefresh;
+    else if (one) out.kind = kWhole;
+    else out.kind = range_uncovered(out.segs, out.n_segs, out.e0, out.e1, c.d.n_valid) ? kRefresh : kMixed;
 }
 
 template <int DT>
@@ -307,7 +337,7 @@ __global__ void __launch_bounds__(kThreads, 1) adam8_kernel(const __grid_constan
                 Slot8 slot;
                 classify<DT>(a, tile_lo + blockIdx.x + k * gridDim.x, skip, cur, slot);
                 s_slot[s] = slot;
-                if (slot.kind == kWhole) {
+                if (slot.kind == kWhole || slot.kind == kMixed) {
                     const int64_t block = slot.e0 / kMomentBlock;
                     mbar_arrive_expect_tx(&s_full[s], S::kLoaded);
                     bulk_g2s(at + S::kP, slot.master + slot.e0, 4 * kTile, &s_full[s]);
@@ -339,9 +369,10 @@ __global__ void __launch_bounds__(kThreads, 1) adam8_kernel(const __grid_constan
                 }
                 const Slot8 slot = s_slot[s];
                 unsigned char* const at = s_dyn + s * S::kBytes;
-                if (slot.kind == kWhole || slot.kind == kRefresh)
+                const bool moments = slot.kind == kWhole || slot.kind == kMixed;
+                if (moments || slot.kind == kRefresh)
                     bulk_s2g(static_cast<T*>(slot.lowp) + slot.e0, at + S::kG, S::kGBytes);
-                if (slot.kind == kWhole) {
+                if (moments) {
                     const int64_t block = slot.e0 / kMomentBlock;
                     bulk_s2g(slot.master + slot.e0, at + S::kP, 4 * kTile);
                     bulk_s2g(slot.state_m + slot.e0, at + S::kM, kTile);
@@ -369,8 +400,7 @@ __global__ void __launch_bounds__(kThreads, 1) adam8_kernel(const __grid_constan
     // the computing warps; the group constants take shape while the first tiles are on their way
     const float div = ctl->div_scale, inv_div = ctl->inv_div;
     const int div_mode = div > 0.0f ? (inv_div != 0.0f ? kMulInv : kTrueDiv) : kNoDiv;
-    if (!skip)
-        for (int gi = threadIdx.x; gi < a.n_groups; gi += kComputing) s_group[gi] = pack_group8(derive_group(a.hyper[gi], step));
+    if (!skip && threadIdx.x < 2 * a.n_groups) derive_half(a.hyper[threadIdx.x >> 1], step, threadIdx.x & 1, s_group[threadIdx.x >> 1]);
     asm volatile("bar.sync 1, %0;" ::"n"(kComputing) : "memory");
 
     float nan_acc = 0.0f;
@@ -389,9 +419,13 @@ __global__ void __launch_bounds__(kThreads, 1) adam8_kernel(const __grid_constan
         T* const sg = reinterpret_cast<T*>(at + S::kG) + warp * kMomentBlock;
         uint8_t *const scm = at + S::kM + warp * kMomentBlock, *const scv = at + S::kV + warp * kMomentBlock;
 
-        if (slot.kind == kWhole) {
-            if (slot.group != have) {
-                have = slot.group;
+        int kind = slot.kind, group = slot.group, seg_lo = 0, seg_hi = -1;
+        if (kind == kMixed && !block_segments(slot.segs, slot.n_segs, slot.seg, a.n_groups, slot.e0 + warp * kMomentBlock,
+                                              slot.e0 + (warp + 1) * kMomentBlock, seg_lo, seg_hi, group))
+            kind = kRefresh;   // this block of it
+        if (kind == kWhole || kind == kMixed) {
+            if (group >= 0 && group != have) {
+                have = group;
                 k8 = s_group[have];
             }
             const int64_t block = slot.e0 / kMomentBlock + warp;
@@ -437,7 +471,7 @@ __global__ void __launch_bounds__(kThreads, 1) adam8_kernel(const __grid_constan
             }
             const uint32_t em = block_exponent(__reduce_max_sync(0xFFFFFFFFu, __float_as_uint(top_m)));
             const uint32_t ev = block_exponent(__reduce_max_sync(0xFFFFFFFFu, __float_as_uint(top_v)));
-            if (max(em, em0) <= kEasyM && max(ev, ev0) <= kEasyV) {
+            if (group >= 0 && max(em, em0) <= kEasyM && max(ev, ev0) <= kEasyV) {
                 const float xm = __uint_as_float((142u - em) << 23);   // 2^(15 - E)
                 const float xv = __uint_as_float((158u - ev) << 23);   // 2^(31 - E)
 #pragma unroll
@@ -474,11 +508,11 @@ __global__ void __launch_bounds__(kThreads, 1) adam8_kernel(const __grid_constan
                 }
             } else {
                 const BlockAt b = {sp, sg, sg, scm, scv, at + S::kEm + warp, at + S::kEv + warp, slot.e0 + warp * kMomentBlock,
-                                   kMomentBlock, nullptr, 0, slot.group};
+                                   kMomentBlock, slot.segs, seg_lo, seg_hi, group};
                 update_block<DT>(b, s_group, a.n_groups, key, div_mode, div, inv_div, nan_acc);
             }
             fence_async_smem();   // the bulk stores read what the threads just wrote
-        } else if (slot.kind == kRefresh) {
+        } else if (kind == kRefresh) {
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
                 const int i = h * 128 + lane * 4;
@@ -487,20 +521,15 @@ __global__ void __launch_bounds__(kThreads, 1) adam8_kernel(const __grid_constan
                 else *reinterpret_cast<uint2*>(sg + i) = make_uint2(Lp<DT>::pack2(pp.x, pp.y), Lp<DT>::pack2(pp.z, pp.w));
             }
             fence_async_smem();
-        } else if (slot.kind == kRagged) {
+        } else if (kind == kRagged) {
             const int64_t b0 = slot.e0 + warp * kMomentBlock, b1 = min(b0 + kMomentBlock, slot.e1);
             T* const lowp = static_cast<T*>(slot.lowp);
             if (b0 < b1) {
-                if (!skip && (slot.group >= 0 || !range_uncovered(slot.segs, slot.n_segs, b0, b1, slot.n_valid))) {
+                if (!skip && (group >= 0 || block_segments(slot.segs, slot.n_segs, slot.seg, a.n_groups, b0, b1, seg_lo, seg_hi, group))) {
                     const int64_t block = b0 / kMomentBlock;
-                    int group = slot.group;
-                    if (group < 0) {   // one segment may cover the block although it does not cover the tile
-                        const int si = find_seg(slot.segs, slot.n_segs, b0);
-                        if (si >= 0 && slot.segs[si].end >= b1 && slot.segs[si].group < a.n_groups) group = slot.segs[si].group;
-                    }
                     const BlockAt b = {slot.master + b0, static_cast<const T*>(slot.gsrc) + b0, lowp + b0, slot.state_m + b0,
                                        slot.state_v + b0, slot.exps_m + block, slot.exps_v + block, b0, static_cast<int>(b1 - b0),
-                                       slot.segs, slot.n_segs, group};
+                                       slot.segs, seg_lo, seg_hi, group};
                     update_block<DT>(b, s_group, a.n_groups, dither_key(step, slot.chunk, block), div_mode, div, inv_div, nan_acc);
                 } else {
                     for (int64_t e = b0 + lane; e < b1; e += 32) lowp[e] = Lp<DT>::from_float(slot.master[e]);
