@@ -18,6 +18,7 @@ namespace {
 struct Group8 {
     float lr, beta1, omb1, beta2, omb2, wd_l2, wd_w;
     float rbc1, rbc2, eps;   // 2^12 / bc1, 2^24 / bc2, 2^12 eps
+    float one;               // 1 (see new_moments2)
 };
 
 // By two threads per group, a moment each: the powers in double are most of a small launch's start.
@@ -36,6 +37,7 @@ __device__ __noinline__ void derive_half(const ElxHyper& h, int step, int second
         k.omb1 = 1.0f - beta;
         k.rbc1 = rbc * 4096.0f;
         k.lr = h.lr;
+        k.one = 1.0f;
         k.eps = h.eps * 4096.0f;
     }
 }
@@ -59,7 +61,7 @@ __device__ __forceinline__ float new_param(float p, float m, float v, const Grou
     float root, inv;
     asm("sqrt.approx.ftz.f32 %0, %1;" : "=f"(root) : "f"(v * k.rbc2));
     asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(inv) : "f"(root + k.eps));
-    return fmaf(-k.lr, fmaf(k.wd_w, p, m * k.rbc1 * inv), p);
+    return fmaf(-k.lr, fmaf(k.wd_w, p, __fmul_rn(__fmul_rn(m, k.rbc1), inv)), p);
 }
 // The same for moments of any size.
 __device__ __noinline__ float new_param_wide(float p, float m, float v, const Group8& k) {
@@ -174,10 +176,58 @@ __device__ __forceinline__ uint32_t byte_to_top(uint32_t w, int j) { return __by
 __device__ __forceinline__ uint32_t top_bytes(uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
     return __byte_perm(__byte_perm(a, b, 0x0073), __byte_perm(c, d, 0x0073), 0x5410);
 }
-__device__ __forceinline__ float max_nan(float a, float b) {
+__device__ __forceinline__ float max_nan(float a, float b, float c) {
     float r;
-    asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+    asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
     return r;
+}
+
+// Two elements per instruction: the packed fp32 operations take one issue slot for both, and issue slots are what the
+// update runs short of first.  The same roundings as new_moments() and new_param().
+// A sum of two products is written as a fused multiply-add of the one product with a 1 that the compiler cannot see
+// through: CUDA 12.9 fuses mul.rn.f32x2 with a following add.rn.f32x2 (as it does the intrinsics for them), which changes
+// the last bit of a moment.
+__device__ __forceinline__ float2 both(float x) { return make_float2(x, x); }
+__device__ __forceinline__ uint64_t as_u64(float2 x) {
+    uint64_t r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(x.x), "f"(x.y));
+    return r;
+}
+__device__ __forceinline__ float2 as_float2(uint64_t x) {
+    float2 r;
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(x));
+    return r;
+}
+__device__ __forceinline__ float2 mul2(float2 x, float2 y) {
+    uint64_t r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(as_u64(x)), "l"(as_u64(y)));
+    return as_float2(r);
+}
+__device__ __forceinline__ float2 add2(float2 x, float2 y) {
+    uint64_t r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(as_u64(x)), "l"(as_u64(y)));
+    return as_float2(r);
+}
+__device__ __forceinline__ float2 fma2(float2 x, float2 y, float2 z) {
+    uint64_t r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(as_u64(x)), "l"(as_u64(y)), "l"(as_u64(z)));
+    return as_float2(r);
+}
+__device__ __forceinline__ void new_moments2(float2 p, float2& m, float2& v, float2 g, const Group8& k, bool l2) {
+    if (l2) g = fma2(both(k.wd_l2), p, g);
+    m = fma2(mul2(both(k.beta1), m), both(k.one), mul2(both(k.omb1), g));
+    v = fma2(mul2(both(k.beta2), v), both(k.one), mul2(mul2(both(k.omb2), g), g));
+}
+__device__ __forceinline__ float2 new_param2(float2 p, float2 m, float2 v, const Group8& k) {
+    const float2 vh = mul2(v, both(k.rbc2));
+    float2 root, inv;
+    asm("sqrt.approx.ftz.f32 %0, %1;" : "=f"(root.x) : "f"(vh.x));
+    asm("sqrt.approx.ftz.f32 %0, %1;" : "=f"(root.y) : "f"(vh.y));
+    const float2 den = add2(root, both(k.eps));
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(inv.x) : "f"(den.x));
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(inv.y) : "f"(den.y));
+    const float2 upd = fma2(both(k.wd_w), p, mul2(mul2(m, both(k.rbc1)), inv));
+    return fma2(both(-k.lr), upd, p);
 }
 
 // ------------------------------------------------------------------------------------------------
@@ -207,6 +257,7 @@ struct Adam8Args {
 constexpr int kWarps = kTile / kMomentBlock;   // 16 computing warps, a block of the tile each
 constexpr int kComputing = 32 * kWarps;
 constexpr int kThreads = kComputing + 32;
+constexpr int kBatch = 16;                     // tiles the mover's lanes look up at a time
 
 template <int DT>
 struct Stage8 {
@@ -305,11 +356,13 @@ __global__ void __launch_bounds__(kThreads, 1) adam8_kernel(const __grid_constan
     constexpr int kStages = S::kStages;
     extern __shared__ __align__(128) unsigned char s_dyn[];
     __shared__ Group8 s_group[kMaxGroups];
-    __shared__ Slot8 s_slot[kStages];
+    __shared__ Slot8 s_slot[2 * kBatch];
+    __shared__ uint32_t s_key[2 * kBatch][kWarps];      // dither keys of the tiles' blocks
     __shared__ __align__(8) uint64_t s_full[kStages];   // the loads of a stage have landed (and its slot is published)
     __shared__ __align__(8) uint64_t s_done[kStages];   // all computing warps are through with a stage
     __shared__ int s_abort;
-    static_assert(kStages * S::kBytes + sizeof(s_group) + sizeof(s_slot) + 2 * sizeof(s_full) + 64 <= 227 * 1024, "shared memory");
+    static_assert(kStages * S::kBytes + sizeof(s_group) + sizeof(s_slot) + sizeof(s_key) + 2 * sizeof(s_full) + 64 <= 227 * 1024,
+                  "shared memory");
 
     ElxCtl* const ctl = a.ctl;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -329,45 +382,64 @@ __global__ void __launch_bounds__(kThreads, 1) adam8_kernel(const __grid_constan
     const int64_t my_tiles = blockIdx.x < a.n_tiles ? (a.n_tiles - blockIdx.x + gridDim.x - 1) / gridDim.x : 0;
 
     if (warp == kWarps) {
-        if (lane == 0) {
-            Cursor8 cur;
-            auto produce = [&](int64_t k) {
-                const int s = static_cast<int>(k % kStages);
-                unsigned char* const at = s_dyn + s * S::kBytes;
+        // The mover: lane 0 issues the copies.  What a tile is (its descriptor, segment, kind and dither keys) is worked out
+        // for 16 tiles at a time, a tile per lane: done tile by tile it held the copies up, a tile being due every 1.4 us.
+        // The slots of the batch before stay in use meanwhile, so there are two batches of them.
+        Cursor8 cur;
+        auto look_up = [&](int64_t k) {
+            if (lane < kBatch && k + lane < my_tiles) {
                 Slot8 slot;
-                classify<DT>(a, tile_lo + blockIdx.x + k * gridDim.x, skip, cur, slot);
-                s_slot[s] = slot;
-                if (slot.kind == kWhole || slot.kind == kMixed) {
-                    const int64_t block = slot.e0 / kMomentBlock;
-                    mbar_arrive_expect_tx(&s_full[s], S::kLoaded);
-                    bulk_g2s(at + S::kP, slot.master + slot.e0, 4 * kTile, &s_full[s]);
-                    bulk_g2s(at + S::kG, static_cast<const T*>(slot.gsrc) + slot.e0, S::kGBytes, &s_full[s]);
-                    bulk_g2s(at + S::kM, slot.state_m + slot.e0, kTile, &s_full[s]);
-                    bulk_g2s(at + S::kV, slot.state_v + slot.e0, kTile, &s_full[s]);
-                    bulk_g2s(at + S::kEm, slot.exps_m + block, kWarps, &s_full[s]);
-                    bulk_g2s(at + S::kEv, slot.exps_v + block, kWarps, &s_full[s]);
-                } else if (slot.kind == kRefresh) {
-                    mbar_arrive_expect_tx(&s_full[s], 4 * kTile);
-                    bulk_g2s(at + S::kP, slot.master + slot.e0, 4 * kTile, &s_full[s]);
-                } else {
-                    mbar_arrive(&s_full[s]);   // nothing to load: publishes the slot
+                classify<DT>(a, tile_lo + blockIdx.x + (k + lane) * gridDim.x, skip, cur, slot);
+                s_slot[(k + lane) % (2 * kBatch)] = slot;
+            }
+            __syncwarp();
+            if (!skip) {
+                for (int i = lane; i < kBatch * kWarps; i += 32) {
+                    const int at = static_cast<int>((k + i / kWarps) % (2 * kBatch));
+                    s_key[at][i % kWarps] = dither_key(step, s_slot[at].chunk, s_slot[at].e0 / kMomentBlock + i % kWarps);
                 }
-            };
-            for (int64_t k = 0; k < my_tiles && k < kStages - 1; ++k) produce(k);
-            int64_t k = 0;
-            for (; k < my_tiles; ++k) {
-                const int s = static_cast<int>(k % kStages);
-                const uint32_t parity = static_cast<uint32_t>((k / kStages) & 1);
-                bool handed_over = false;
-                for (uint32_t i = 0; i < kTmaSpinLimit && !handed_over; ++i) {
-                    handed_over = mbar_try_wait(&s_done[s], parity);
-                    if (!handed_over && *reinterpret_cast<volatile int*>(&s_abort)) break;
-                }
-                if (!handed_over) {
-                    s_abort = 1;
-                    break;
-                }
-                const Slot8 slot = s_slot[s];
+            }
+            __syncwarp();
+        };
+        auto produce = [&](int64_t k, int s) {
+            if (k % kBatch == 0) look_up(k);
+            if (lane != 0) return;
+            unsigned char* const at = s_dyn + s * S::kBytes;
+            const Slot8& slot = s_slot[k % (2 * kBatch)];
+            if (slot.kind == kWhole || slot.kind == kMixed) {
+                const int64_t block = slot.e0 / kMomentBlock;
+                mbar_arrive_expect_tx(&s_full[s], S::kLoaded);
+                bulk_g2s(at + S::kP, slot.master + slot.e0, 4 * kTile, &s_full[s]);
+                bulk_g2s(at + S::kG, static_cast<const T*>(slot.gsrc) + slot.e0, S::kGBytes, &s_full[s]);
+                bulk_g2s(at + S::kM, slot.state_m + slot.e0, kTile, &s_full[s]);
+                bulk_g2s(at + S::kV, slot.state_v + slot.e0, kTile, &s_full[s]);
+                bulk_g2s(at + S::kEm, slot.exps_m + block, kWarps, &s_full[s]);
+                bulk_g2s(at + S::kEv, slot.exps_v + block, kWarps, &s_full[s]);
+            } else if (slot.kind == kRefresh) {
+                mbar_arrive_expect_tx(&s_full[s], 4 * kTile);
+                bulk_g2s(at + S::kP, slot.master + slot.e0, 4 * kTile, &s_full[s]);
+            } else {
+                mbar_arrive(&s_full[s]);   // nothing to load: publishes the slot
+            }
+        };
+        for (int k = 0; k < my_tiles && k < kStages - 1; ++k) produce(k, k);
+        int64_t k = 0;
+        int s = 0;
+        uint32_t parity = 0;
+        bool gave_up = false;
+        for (; k < my_tiles; ++k) {
+            bool handed_over = false;
+            for (uint32_t i = 0; i < kTmaSpinLimit && !handed_over; ++i) {
+                handed_over = mbar_try_wait(&s_done[s], parity);
+                if (!handed_over && *reinterpret_cast<volatile int*>(&s_abort)) break;
+            }
+            gave_up = __any_sync(0xFFFFFFFFu, !handed_over);
+            if (gave_up) {
+                s_abort = 1;
+                break;
+            }
+            if (lane == 0) {
+                const Slot8& slot = s_slot[k % (2 * kBatch)];
                 unsigned char* const at = s_dyn + s * S::kBytes;
                 const bool moments = slot.kind == kWhole || slot.kind == kMixed;
                 if (moments || slot.kind == kRefresh)
@@ -381,12 +453,19 @@ __global__ void __launch_bounds__(kThreads, 1) adam8_kernel(const __grid_constan
                     bulk_s2g(slot.exps_v + block, at + S::kEv, kWarps);
                 }
                 bulk_commit();
-                if (k + kStages - 1 < my_tiles) {
-                    bulk_wait_read<1>();   // the stage of tile k-1 has been read out by its stores
-                    produce(k + kStages - 1);
-                }
             }
-            if (s_abort) {
+            const int before = s == 0 ? kStages - 1 : s - 1;
+            if (k + kStages - 1 < my_tiles) {
+                if (lane == 0) bulk_wait_read<1>();   // the stage of tile k-1 has been read out by its stores
+                produce(k + kStages - 1, before);
+            }
+            if (++s == kStages) {
+                s = 0;
+                parity ^= 1u;
+            }
+        }
+        if (lane == 0) {
+            if (gave_up) {
                 // the loads already issued still target this CTA's shared memory: wait (bounded again) for them
                 for (int64_t j = k; j < my_tiles && j < k + kStages - 1; ++j)
                     (void)mbar_wait_bounded(&s_full[j % kStages], static_cast<uint32_t>((j / kStages) & 1));
@@ -407,13 +486,16 @@ __global__ void __launch_bounds__(kThreads, 1) adam8_kernel(const __grid_constan
     bool bad_desc = false;
     Group8 k8 = {};
     int have = -1;
+    bool l2 = false;
+    int s = 0;
+    uint32_t parity = 0;
     for (int64_t k = 0; k < my_tiles; ++k) {
-        const int s = static_cast<int>(k % kStages);
-        if (!mbar_wait_bounded(&s_full[s], static_cast<uint32_t>((k / kStages) & 1)) || *reinterpret_cast<volatile int*>(&s_abort)) {
+        if (!mbar_wait_bounded(&s_full[s], parity)) {
             s_abort = 1;
             break;
         }
-        const Slot8& slot = s_slot[s];
+        const int slot_at = static_cast<int>(k) & (2 * kBatch - 1);
+        const Slot8& slot = s_slot[slot_at];
         unsigned char* const at = s_dyn + s * S::kBytes;
         float* const sp = reinterpret_cast<float*>(at + S::kP) + warp * kMomentBlock;
         T* const sg = reinterpret_cast<T*>(at + S::kG) + warp * kMomentBlock;
@@ -427,12 +509,12 @@ __global__ void __launch_bounds__(kThreads, 1) adam8_kernel(const __grid_constan
             if (group >= 0 && group != have) {
                 have = group;
                 k8 = s_group[have];
+                l2 = k8.wd_l2 != 0.0f;
             }
-            const int64_t block = slot.e0 / kMomentBlock + warp;
-            const uint32_t key = dither_key(step, slot.chunk, block);
+            const uint32_t key = s_key[slot_at][warp];
             const uint32_t em0 = at[S::kEm + warp], ev0 = at[S::kEv + warp];
             // a lane owns 2 x 4 consecutive elements, 128 apart: conflict-free accesses of whole words
-            float p[8], m[8], v[8];
+            float2 p[4], m[4], v[4];
             const float dm = em0 ? __uint_as_float((em0 + 112u) << 23) : 0.0f;   // 2^(E - 15)
             const float dv = ev0 ? __uint_as_float((ev0 + 96u) << 23) : 0.0f;    // 2^(E - 31)
             float top_m = 0.0f, top_v = 0.0f;
@@ -441,32 +523,36 @@ __global__ void __launch_bounds__(kThreads, 1) adam8_kernel(const __grid_constan
                 const int i = h * 128 + lane * 4;
                 const float4 pp = *reinterpret_cast<const float4*>(sp + i);
                 const uint32_t cm = *reinterpret_cast<const uint32_t*>(scm + i), cv = *reinterpret_cast<const uint32_t*>(scv + i);
-                float g[4];
+                float2 g[2];
                 if constexpr (DT == ELX_F32) {
                     const float4 gg = *reinterpret_cast<const float4*>(sg + i);
-                    g[0] = gg.x; g[1] = gg.y; g[2] = gg.z; g[3] = gg.w;
+                    g[0] = make_float2(gg.x, gg.y);
+                    g[1] = make_float2(gg.z, gg.w);
                 } else {
                     const uint2 gg = *reinterpret_cast<const uint2*>(sg + i);
-                    const float2 a0 = Lp<DT>::unpack2(gg.x), a1 = Lp<DT>::unpack2(gg.y);
-                    g[0] = a0.x; g[1] = a0.y; g[2] = a1.x; g[3] = a1.y;
+                    g[0] = Lp<DT>::unpack2(gg.x);
+                    g[1] = Lp<DT>::unpack2(gg.y);
                 }
-                p[4 * h] = pp.x; p[4 * h + 1] = pp.y; p[4 * h + 2] = pp.z; p[4 * h + 3] = pp.w;
+                p[2 * h] = make_float2(pp.x, pp.y);
+                p[2 * h + 1] = make_float2(pp.z, pp.w);
                 if (div_mode == kMulInv) {
 #pragma unroll
-                    for (int j = 0; j < 4; ++j) g[j] *= inv_div;
+                    for (int j = 0; j < 2; ++j) g[j] = mul2(g[j], both(inv_div));
                 } else if (div_mode == kTrueDiv) {
 #pragma unroll
-                    for (int j = 0; j < 4; ++j) g[j] = div_or_zero(g[j], div);
+                    for (int j = 0; j < 2; ++j) g[j] = make_float2(div_or_zero(g[j].x, div), div_or_zero(g[j].y, div));
                 }
 #pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    const int q = 4 * h + j;
-                    const uint32_t bm = byte_to_top(cm, j), bv = byte_to_top(cv, j);
-                    m[q] = __uint_as_float((static_cast<uint32_t>(static_cast<int32_t>(bm) >> 4) & 0x87F00000u)) * dm;
-                    v[q] = __uint_as_float(bv >> 4) * dv;
-                    new_moments(p[q], m[q], v[q], g[j], k8);
-                    top_m = max_nan(top_m, fabsf(m[q]));
-                    top_v = max_nan(top_v, v[q]);
+                for (int j = 0; j < 2; ++j) {
+                    const int q = 2 * h + j;
+                    // sign and magnitude from the two ends of the byte, moved down by 4 to where fp32 has them
+                    const int32_t m0 = static_cast<int32_t>(byte_to_top(cm, 2 * j)), m1 = static_cast<int32_t>(byte_to_top(cm, 2 * j + 1));
+                    m[q] = mul2(make_float2(__int_as_float((m0 >> 4) & 0x87F00000), __int_as_float((m1 >> 4) & 0x87F00000)), both(dm));
+                    v[q] = mul2(make_float2(__uint_as_float(byte_to_top(cv, 2 * j) >> 4),
+                                                  __uint_as_float(byte_to_top(cv, 2 * j + 1) >> 4)), both(dv));
+                    new_moments2(p[q], m[q], v[q], g[j], k8, l2);
+                    top_m = max_nan(top_m, fabsf(m[q].x), fabsf(m[q].y));
+                    top_v = max_nan(top_v, v[q].x, v[q].y);
                 }
             }
             const uint32_t em = block_exponent(__reduce_max_sync(0xFFFFFFFFu, __float_as_uint(top_m)));
@@ -479,26 +565,31 @@ __global__ void __launch_bounds__(kThreads, 1) adam8_kernel(const __grid_constan
                     const int i = h * 128 + lane * 4;
                     uint32_t tm[4], tv[4];
 #pragma unroll
-                    for (int j = 0; j < 4; ++j) {
-                        const int q = 4 * h + j;
-                        const uint32_t r = dither_bits(key, i + j);
-                        // the kept bits of a code end at bit 24 after a shift by 4: the code is the top byte
-                        // (__fmul_rn and the masks are deliberate: nvcc 12.9 gets a plain product followed by byte
-                        // permutes of the dither wrong here -- all codes 0 -- and the tests of the codes show it)
-                        tm[j] = (__float_as_uint(__fmul_rn(fabsf(m[q]), xm)) << 4) + ((r & 0xFFFFu) << 8);
-                        tm[j] = (__float_as_uint(m[q]) & 0x80000000u) | tm[j];
-                        tv[j] = (__float_as_uint(__fmul_rn(v[q], xv)) << 4) + ((r >> 16) << 8);
-                        if (v[q] > 0.0f) tv[j] = max(tv[j], 0x1000000u);
-                        p[q] = new_param(p[q], m[q], v[q], k8);
+                    for (int j = 0; j < 2; ++j) {
+                        const int q = 2 * h + j;
+                        const float2 zm = mul2(m[q], both(xm)), zv = mul2(v[q], both(xv));
+                        const uint32_t r0 = dither_bits(key, i + 2 * j), r1 = dither_bits(key, i + 2 * j + 1);
+                        // a shift by 4 drops the sign and lets the kept bits of a code end at bit 24: the code is the top byte
+                        tm[2 * j] = ((__float_as_uint(zm.x) << 4) + __byte_perm(r0, 0, 0x4104)) | (__float_as_uint(zm.x) & 0x80000000u);
+                        tm[2 * j + 1] = ((__float_as_uint(zm.y) << 4) + __byte_perm(r1, 0, 0x4104)) | (__float_as_uint(zm.y) & 0x80000000u);
+                        tv[2 * j] = (__float_as_uint(zv.x) << 4) + __byte_perm(r0, 0, 0x4324);
+                        tv[2 * j + 1] = (__float_as_uint(zv.y) << 4) + __byte_perm(r1, 0, 0x4324);
+                        p[q] = new_param2(p[q], m[q], v[q], k8);
+                    }
+                    if (min(min(tv[0], tv[1]), min(tv[2], tv[3])) < 0x1000000u) {   // a code 0 stays only for a moment of 0
+                        if (v[2 * h].x > 0.0f) tv[0] = max(tv[0], 0x1000000u);
+                        if (v[2 * h].y > 0.0f) tv[1] = max(tv[1], 0x1000000u);
+                        if (v[2 * h + 1].x > 0.0f) tv[2] = max(tv[2], 0x1000000u);
+                        if (v[2 * h + 1].y > 0.0f) tv[3] = max(tv[3], 0x1000000u);
                     }
                     *reinterpret_cast<uint32_t*>(scm + i) = top_bytes(tm[0], tm[1], tm[2], tm[3]);
                     *reinterpret_cast<uint32_t*>(scv + i) = top_bytes(tv[0], tv[1], tv[2], tv[3]);
-                    *reinterpret_cast<float4*>(sp + i) = make_float4(p[4 * h], p[4 * h + 1], p[4 * h + 2], p[4 * h + 3]);
+                    *reinterpret_cast<float4*>(sp + i) = make_float4(p[2 * h].x, p[2 * h].y, p[2 * h + 1].x, p[2 * h + 1].y);
                     if constexpr (DT == ELX_F32) {
-                        *reinterpret_cast<float4*>(sg + i) = make_float4(p[4 * h], p[4 * h + 1], p[4 * h + 2], p[4 * h + 3]);
+                        *reinterpret_cast<float4*>(sg + i) = make_float4(p[2 * h].x, p[2 * h].y, p[2 * h + 1].x, p[2 * h + 1].y);
                     } else {
-                        *reinterpret_cast<uint2*>(sg + i) = make_uint2(Lp<DT>::pack2(p[4 * h], p[4 * h + 1]),
-                                                                       Lp<DT>::pack2(p[4 * h + 2], p[4 * h + 3]));
+                        *reinterpret_cast<uint2*>(sg + i) = make_uint2(Lp<DT>::pack2(p[2 * h].x, p[2 * h].y),
+                                                                       Lp<DT>::pack2(p[2 * h + 1].x, p[2 * h + 1].y));
                     }
                 }
                 __syncwarp();   // every lane has read the old exponents
@@ -530,7 +621,7 @@ __global__ void __launch_bounds__(kThreads, 1) adam8_kernel(const __grid_constan
                     const BlockAt b = {slot.master + b0, static_cast<const T*>(slot.gsrc) + b0, lowp + b0, slot.state_m + b0,
                                        slot.state_v + b0, slot.exps_m + block, slot.exps_v + block, b0, static_cast<int>(b1 - b0),
                                        slot.segs, seg_lo, seg_hi, group};
-                    update_block<DT>(b, s_group, a.n_groups, dither_key(step, slot.chunk, block), div_mode, div, inv_div, nan_acc);
+                    update_block<DT>(b, s_group, a.n_groups, s_key[slot_at][warp], div_mode, div, inv_div, nan_acc);
                 } else {
                     for (int64_t e = b0 + lane; e < b1; e += 32) lowp[e] = Lp<DT>::from_float(slot.master[e]);
                 }
@@ -540,6 +631,10 @@ __global__ void __launch_bounds__(kThreads, 1) adam8_kernel(const __grid_constan
         }
         __syncwarp();
         if (lane == 0) mbar_arrive(&s_done[s]);
+        if (++s == kStages) {
+            s = 0;
+            parity ^= 1u;
+        }
     }
 
     const unsigned late = __ballot_sync(0xFFFFFFFFu, nan_acc != nan_acc);
