@@ -187,32 +187,6 @@ __device__ __forceinline__ float max_nan(float a, float b, float c) {
 // A sum of two products is written as a fused multiply-add of the one product with a 1 that the compiler cannot see
 // through: CUDA 12.9 fuses mul.rn.f32x2 with a following add.rn.f32x2 (as it does the intrinsics for them), which changes
 // the last bit of a moment.
-__device__ __forceinline__ float2 both(float x) { return make_float2(x, x); }
-__device__ __forceinline__ uint64_t as_u64(float2 x) {
-    uint64_t r;
-    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(x.x), "f"(x.y));
-    return r;
-}
-__device__ __forceinline__ float2 as_float2(uint64_t x) {
-    float2 r;
-    asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(x));
-    return r;
-}
-__device__ __forceinline__ float2 mul2(float2 x, float2 y) {
-    uint64_t r;
-    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(as_u64(x)), "l"(as_u64(y)));
-    return as_float2(r);
-}
-__device__ __forceinline__ float2 add2(float2 x, float2 y) {
-    uint64_t r;
-    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(as_u64(x)), "l"(as_u64(y)));
-    return as_float2(r);
-}
-__device__ __forceinline__ float2 fma2(float2 x, float2 y, float2 z) {
-    uint64_t r;
-    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(as_u64(x)), "l"(as_u64(y)), "l"(as_u64(z)));
-    return as_float2(r);
-}
 __device__ __forceinline__ void new_moments2(float2 p, float2& m, float2& v, float2 g, const Group8& k, bool l2) {
     if (l2) g = fma2(both(k.wd_l2), p, g);
     m = fma2(mul2(both(k.beta1), m), both(k.one), mul2(both(k.omb1), g));

@@ -172,6 +172,41 @@ __device__ __forceinline__ void st_words(void* p, const uint32_t (&w)[N]) {
 }
 
 // ------------------------------------------------------------------------------------------------
+// packed fp32 arithmetic: two elements per instruction (and per issue slot)
+// ------------------------------------------------------------------------------------------------
+
+__device__ __forceinline__ float2 both(float x) { return make_float2(x, x); }
+__device__ __forceinline__ uint64_t as_u64(float2 x) {
+    uint64_t r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(x.x), "f"(x.y));
+    return r;
+}
+__device__ __forceinline__ float2 as_float2(uint64_t x) {
+    float2 r;
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(x));
+    return r;
+}
+__device__ __forceinline__ float2 mul2(float2 x, float2 y) {
+    uint64_t r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(as_u64(x)), "l"(as_u64(y)));
+    return as_float2(r);
+}
+__device__ __forceinline__ float2 add2(float2 x, float2 y) {
+    uint64_t r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(as_u64(x)), "l"(as_u64(y)));
+    return as_float2(r);
+}
+__device__ __forceinline__ float2 fma2(float2 x, float2 y, float2 z) {
+    uint64_t r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(as_u64(x)), "l"(as_u64(y)), "l"(as_u64(z)));
+    return as_float2(r);
+}
+// The same names for one element, for code that is written for either.
+__device__ __forceinline__ float mul2(float x, float y) { return x * y; }
+__device__ __forceinline__ float add2(float x, float y) { return x + y; }
+__device__ __forceinline__ float fma2(float x, float y, float z) { return fmaf(x, y, z); }
+
+// ------------------------------------------------------------------------------------------------
 // low-precision element traits
 // ------------------------------------------------------------------------------------------------
 
