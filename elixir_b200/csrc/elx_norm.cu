@@ -166,6 +166,16 @@ __device__ __forceinline__ float warp_sum(float v) {
     return v;
 }
 
+// Sums of two values over a warp: half of the lanes take over one of them first, 6 exchanges instead of 10.  Lanes 0 to 15
+// end up with the first sum, the others with the second.
+__device__ __forceinline__ float warp_sum_pair(float a, float b) {
+    const bool high = threadIdx.x & 16;
+    float v = (high ? b : a) + __shfl_xor_sync(0xFFFFFFFFu, high ? a : b, 16);
+#pragma unroll
+    for (int o = 8; o > 0; o >>= 1) v += __shfl_xor_sync(0xFFFFFFFFu, v, o);
+    return v;
+}
+
 // Sums of N values over the threads of a block; every thread gets them.  s: N * 32 floats, not used by another sum
 // between two barriers.
 template <int N>
@@ -423,7 +433,12 @@ __global__ void __launch_bounds__(512, 1) norm_backward_kernel(const NormArgs a)
     const int groups = blockDim.x / threads, warps = threads >> 5, warp = t >> 5;
     using V = Values<VEC>;
     using E = typename V::E;
-    Piece<DT, VEC> w[NEXT ? VPL : 1], x[VPL], dy[VPL], nx[NEXT ? VPL : 1], ndy[NEXT ? VPL : 1];
+    // KEPT (fp32): differences and products of a row's first half stay in registers for the second, and the next row is asked
+    // for in between.  Else both are formed again from the row as it is held, and the next row is asked for at once: 16-bit
+    // rows hold twice the elements in those registers (8192 x 1600: fp32 37 us against 49, fp16 24.5 us against 24.8;
+    // 16384 x 4096 bf16 107 us against 79).
+    constexpr bool KEPT = NEXT && DT == ELX_F32, EARLY = NEXT && !KEPT;
+    Piece<DT, VEC> w[NEXT ? VPL : 1], x[VPL], dy[VPL], nx[EARLY ? VPL : 1], ndy[EARLY ? VPL : 1];
     E dw[VPL][V::kN], db[VPL][V::kN];
     const int64_t stride = static_cast<int64_t>(gridDim.x) * groups, total = a.rows * a.cols;
     int64_t row = static_cast<int64_t>(blockIdx.x) * groups + group;
@@ -439,6 +454,10 @@ __global__ void __launch_bounds__(512, 1) norm_backward_kernel(const NormArgs a)
         }
         x[i].zero();
         dy[i].zero();
+        if constexpr (EARLY) {
+            nx[i].zero();
+            ndy[i].zero();
+        }
         if constexpr (NEXT) {
             w[i].zero();
             if constexpr (ODD) {
@@ -447,15 +466,11 @@ __global__ void __launch_bounds__(512, 1) norm_backward_kernel(const NormArgs a)
                 if (a.weight && span[i].any) w[i].load(a.weight, span[i].c);
             }
         }
-        if constexpr (NEXT) {
-            nx[i].zero();
-            ndy[i].zero();
-        }
 #pragma unroll
         for (int j = 0; j < V::kN; ++j) dw[i][j] = db[i][j] = V::all(0.0f);
     }
     const float inv = 1.0f / static_cast<float>(a.cols);
-    float mean = 0.0f, rstd = 0.0f, next_mean = 0.0f, next_rstd = 0.0f;
+    float mean = 0.0f, rstd = 0.0f;
     auto fetch = [&](int64_t r, Piece<DT, VEC>* px, Piece<DT, VEC>* pdy, float& m, float& s) {
         m = a.mean[r];
         s = a.rstd[r];
@@ -483,12 +498,14 @@ __global__ void __launch_bounds__(512, 1) norm_backward_kernel(const NormArgs a)
         }
     };
     if (NEXT && row < a.rows) fetch(row, x, dy, mean, rstd);
+    float next_mean = 0.0f, next_rstd = 0.0f;
+    E d[KEPT ? VPL : 1][V::kN], g[KEPT ? VPL : 1][V::kN];
     for (int parity = 0; row < a.rows; row += stride, parity ^= 1) {
-        if constexpr (NEXT) {
+        if constexpr (!NEXT) fetch(row, x, dy, mean, rstd);
+        if constexpr (EARLY) {
             if (row + stride < a.rows) fetch(row + stride, nx, ndy, next_mean, next_rstd);
-        } else {
-            fetch(row, x, dy, mean, rstd);
         }
+        const float now_rstd = rstd;
         const E scale = V::all(rstd), minus = V::all(-mean);
         E sum0 = V::all(0.0f), sum1 = V::all(0.0f), fx[V::kN], fd[V::kN], fw[V::kN];
 #pragma unroll
@@ -503,20 +520,26 @@ __global__ void __launch_bounds__(512, 1) norm_backward_kernel(const NormArgs a)
             weights(i, fw);
 #pragma unroll
             for (int j = 0; j < V::kN; ++j) {
-                const E xhat = mul2(add2(fx[j], minus), scale);
+                const E diff = add2(fx[j], minus), xhat = mul2(diff, scale);
                 dw[i][j] = fma2(fd[j], xhat, dw[i][j]);
                 db[i][j] = add2(db[i][j], fd[j]);
-                const E g = a.weight ? mul2(fd[j], fw[j]) : fd[j];
-                sum0 = add2(sum0, g);
-                sum1 = fma2(g, xhat, sum1);
+                const E prod = a.weight ? mul2(fd[j], fw[j]) : fd[j];
+                sum0 = add2(sum0, prod);
+                sum1 = fma2(prod, xhat, sum1);
+                if constexpr (KEPT) {
+                    d[i][j] = diff;
+                    g[i][j] = prod;
+                }
             }
         }
-        float2 sum = make_float2(V::sum(sum0), V::sum(sum1));
-        sum.x = warp_sum(sum.x);
-        sum.y = warp_sum(sum.y);
+        if constexpr (KEPT) {
+            if (row + stride < a.rows) fetch(row + stride, x, dy, mean, rstd);
+        }
+        const float pair = warp_sum_pair(V::sum(sum0), V::sum(sum1));
+        float2 sum;
         if (warps > 1) {
             // one barrier per row: the next row writes the other half, and the row after it only past the next barrier
-            if ((t & 31) == 0) s_sum[parity][group][warp] = sum;
+            if ((t & 15) == 0) reinterpret_cast<float*>(&s_sum[parity][group][warp])[(t >> 4) & 1] = pair;
             asm volatile("bar.sync %0, %1;" ::"r"(1 + group), "r"(threads) : "memory");
             sum = s_sum[parity][group][0];
             for (int j = 1; j < warps; ++j) {
@@ -524,26 +547,35 @@ __global__ void __launch_bounds__(512, 1) norm_backward_kernel(const NormArgs a)
                 sum.x += o.x;
                 sum.y += o.y;
             }
+        } else {
+            sum.x = __shfl_sync(0xFFFFFFFFu, pair, 0);
+            sum.y = __shfl_sync(0xFFFFFFFFu, pair, 16);
         }
         // dx = rstd (g - m0 - (x - mean) rstd m1): exactly zero where there is nothing to spread over
-        const E m0 = V::all(-(sum.x * inv)), m1 = V::all(-(sum.y * inv) * rstd);
+        const E m0 = V::all(-(sum.x * inv)), m1 = V::all(-(sum.y * inv) * now_rstd);
 #pragma unroll
         for (int i = 0; i < VPL; ++i) {
             if (!span[i].any) continue;
-            x[i].get(fx);
-            dy[i].get(fd);
-            weights(i, fw);
+            if constexpr (!KEPT) {
+                x[i].get(fx);
+                dy[i].get(fd);
+                weights(i, fw);
+            }
 #pragma unroll
             for (int j = 0; j < V::kN; ++j) {
-                const E g = a.weight ? mul2(fd[j], fw[j]) : fd[j];
-                fd[j] = mul2(scale, fma2(add2(fx[j], minus), m1, add2(g, m0)));
+                if constexpr (KEPT) {
+                    fd[j] = mul2(scale, fma2(d[i][j], m1, add2(g[i][j], m0)));
+                } else {
+                    const E prod = a.weight ? mul2(fd[j], fw[j]) : fd[j];
+                    fd[j] = mul2(scale, fma2(add2(fx[j], minus), m1, add2(prod, m0)));
+                }
             }
             Piece<DT, VEC> out;
             out.put(fd);
             if constexpr (ODD) store_span<DT, VEC>(out, a.out, span[i], row * a.cols + span[i].c, a.cols);
             else out.store(a.out, row * a.cols + span[i].c);
         }
-        if constexpr (NEXT) {
+        if constexpr (EARLY) {
 #pragma unroll
             for (int i = 0; i < VPL; ++i) {
                 x[i] = nx[i];
