@@ -303,10 +303,10 @@ __device__ __forceinline__ float group_sum(float v, float* s, int id, int thread
 
 // Rows of a width that 16-byte pieces do not divide.  Groups of threads walk over rows that all begin at one distance from
 // a 16-byte boundary (their number is a multiple of V), so a thread's columns, weights and biases stay the same, and x and y
-// move in 16-byte pieces but for the two ends of a row: 8192 x 1111 fp16 in 15 us instead of 31 us with an access per
-// element.
+// move in 16-byte pieces but for the two ends of a row.  8192 x 1111: fp16 24 us (31 us with an access per element), and
+// 8192 x 1601 fp32 37 us.  Bound by instructions: 31 per element, half of them for the ends of the rows.
 template <int DT, int VPL>
-__global__ void __launch_bounds__(512, 1) norm_forward_odd_kernel(const NormArgs a) {
+__global__ void __launch_bounds__(512, VPL > 2 ? 1 : 2) norm_forward_odd_kernel(const NormArgs a) {
     constexpr int VEC = Wide<DT>::kVec;
     __shared__ float s_sum[2][2][16][16];   // [row parity][which sum][group][warp]
     const int threads = a.group_threads, group = threadIdx.x / threads, t = threadIdx.x - group * threads;
@@ -744,7 +744,7 @@ int launch_forward_odd(NormArgs a, cudaStream_t s) {
     a.group_threads = round32((pieces + VPL - 1) / VPL);
     int per_block = 512 / a.group_threads;
     if (per_block > 15 && a.group_threads > 32) per_block = 15;   // named barriers
-    const int blocks = row_blocks((a.rows + per_block - 1) / per_block, per_block, V);
+    const int each = VPL > 2 ? 1 : 2, blocks = each * row_blocks((a.rows + per_block * each - 1) / (per_block * each), per_block, V);
     norm_forward_odd_kernel<DT, VPL><<<blocks, per_block * a.group_threads, 0, s>>>(a);
     return record_cuda(cudaGetLastError());
 }
@@ -757,7 +757,7 @@ int forward_dt(const NormArgs& a, bool wide_ok, bool same_mis, cudaStream_t s) {
     if (!wide_ok && same_mis && a.cols >= 4 * V) {
         const int pieces = (a.cols + 2 * V - 2) / V;
         if (pieces <= 32) return launch_forward_odd<DT, 1>(a, s);
-        if (pieces <= 64) return launch_forward_odd<DT, 2>(a, s);
+        if (pieces <= 512) return launch_forward_odd<DT, 2>(a, s);
         if (pieces <= 2048) return launch_forward_odd<DT, 4>(a, s);
     }
     const int warps = wide_ok ? forward_warps<V>(a.cols / V, &each) : forward_warps<1>(a.cols, &each);
