@@ -545,8 +545,8 @@ int elx_adam8_multi(const ElxChunkDesc* descs, int first, int count, int64_t n_t
 /*
  * Both moments of a shard into the 8-bit form (rounded to nearest) and back.  exp_avg, exp_avg_sq: device, n floats
  * (unpack: n elements of `dtype`, ELX_F32 or ELX_BF16; bf16 holds every value from 2^-126 up exactly).  state_m,
- * state_v: device, elx_moment_state_bytes(n) bytes; pack leaves the padding bytes as they are.  The sign of exp_avg_sq
- * is dropped.  For checkpoints that hold fp32 moments, and for readers of the state.
+ * state_v: device, elx_moment_state_bytes(n) bytes; pack writes the padding bytes as zeros.  The sign of exp_avg_sq is
+ * dropped.  For checkpoints that hold fp32 moments, and for readers of the state.
  */
 int elx_moments_pack(const float* exp_avg, const float* exp_avg_sq, int64_t n, void* state_m, void* state_v, void* stream);
 int elx_moments_unpack(const void* state_m, const void* state_v, int64_t n, int dtype, void* exp_avg, void* exp_avg_sq,
@@ -578,8 +578,9 @@ int elx_layer_norm_backward(const void* dy, const void* x, const void* weight, c
  * 8, signed) bytes each, and its gradient dweight[v] = scale * sum of dout[i] over the i with tokens[i] == v: dense,
  * every row written, zero where no token points.  The sum is fp32, in ascending order within pieces whose borders the
  * tokens alone fix, so it is the same for every run.  Tokens equal to padding_idx (-1 = none) add to no row.  A token
- * outside [0, vocab) reads as a row of NaN and adds to no row.  workspace: elx_embedding_backward_workspace(n, width)
- * bytes, 16-byte aligned, not shared with a call that may run at the same time.
+ * outside [0, vocab) reads as a row of NaN and adds to no row.  n and vocab below 2^31, width below 2^30.  workspace:
+ * elx_embedding_backward_workspace(n, width) bytes, 16-byte aligned, not shared with a call that may run at the same
+ * time.
  */
 int elx_embedding_forward(const void* tokens, int index_bytes, int64_t n, const void* weight, int dtype, int64_t vocab,
                           int64_t width, float scale, void* out, void* stream);

@@ -43,7 +43,7 @@ def test_embedding_entry_points_reject_bad_arguments(native):
     assert fwd(t=None) == fwd(w=None) == fwd(o=None) == E.ERR_NULL
     assert fwd(ib=2) == fwd(dt=9) == E.ERR_DTYPE
     assert fwd(n=-1) == fwd(v=0) == fwd(h=0) == E.ERR_SIZE
-    assert fwd(n=2**31) == fwd(v=2**31) == E.ERR_CAPACITY
+    assert fwd(n=2**31) == fwd(v=2**31) == fwd(h=2**30) == E.ERR_CAPACITY
     assert fwd(t=ctypes.c_void_p(68)) == fwd(w=odd) == fwd(o=odd) == E.ERR_ALIGN
     assert fwd(n=0, t=None, o=None) == E.OK
     need = lib.elx_embedding_backward_workspace(4, 8)
