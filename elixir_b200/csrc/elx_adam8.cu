@@ -718,6 +718,11 @@ __global__ void __launch_bounds__(kConvThreads) pack_kernel(const float* __restr
             }
         }
     }
+    if (blockIdx.x == 0 && threadIdx.x < 32) {   // the padding: fewer than 16 bytes behind the codes and behind the exponents
+        const int64_t exps = moment_exps_at(n), end = exps + (n + kMomentBlock - 1) / kMomentBlock;
+        const int64_t at = threadIdx.x < 16 ? n + threadIdx.x : end + threadIdx.x - 16;
+        if (at < (threadIdx.x < 16 ? exps : moment_state_bytes(n))) state_m[at] = state_v[at] = 0;
+    }
 }
 
 template <class M, int DT>

@@ -695,7 +695,7 @@ def moment_state_bytes(n: int) -> int:
 
 def _same_device(*named):
     index = named[0][1].get_device()
-    for name, t in named[1:]:
+    for name, t in named:
         if t is not None and t.get_device() != index:
             raise ValueError(f'{name} is on {t.device}, {named[0][0]} on {named[0][1].device}')
 
@@ -715,9 +715,9 @@ def pack_moments(exp_avg: torch.Tensor, exp_avg_sq: torch.Tensor, state_m: Optio
         raise ValueError('the two moments differ in size')
     size = moment_state_bytes(n)
     if state_m is None:
-        state_m = torch.zeros(size, dtype=torch.uint8, device=exp_avg.device)
+        state_m = torch.empty(size, dtype=torch.uint8, device=exp_avg.device)
     if state_v is None:
-        state_v = torch.zeros(size, dtype=torch.uint8, device=exp_avg.device)
+        state_v = torch.empty(size, dtype=torch.uint8, device=exp_avg.device)
     for name, t in (('state_m', state_m), ('state_v', state_v)):
         _check_tensor(t, name, torch.uint8)
         if t.numel() != size:
@@ -775,8 +775,8 @@ def layer_norm_forward(x: torch.Tensor, weight: Optional[torch.Tensor] = None, b
     fp32, the mean and the reciprocal standard deviation that ``layer_norm_backward`` takes."""
     rows, cols = _check_norm(x, weight, bias)
     y = torch.empty_like(x)
-    mean = torch.empty(rows, dtype=torch.float32, device=x.device)
-    rstd = torch.empty_like(mean)
+    mean = x.new_empty(rows, dtype=torch.float32)
+    rstd = mean.new_empty(rows)
     if rows:
         _call('elx_layer_norm_forward', x, x.data_ptr(), _addr(weight), _addr(bias), dtype_code(x.dtype), rows, cols, eps,
               y.data_ptr(), mean.data_ptr(), rstd.data_ptr())
@@ -822,12 +822,11 @@ def embedding_forward(tokens: torch.Tensor, weight: torch.Tensor, scale: float =
     if weight.dim() != 2 or weight.numel() == 0:
         raise ValueError('weight must be a table of at least one row and one column')
     _same_device(('weight', weight), ('tokens', tokens))
-    code = dtype_code(weight.dtype)
-    out = torch.empty(tokens.shape + weight.shape[1:], dtype=weight.dtype, device=weight.device)
-    n = tokens.numel()
+    code, (vocab, width), n = dtype_code(weight.dtype), weight.shape, tokens.numel()
+    out = weight.new_empty((*tokens.shape, width))
     if n:
-        _call('elx_embedding_forward', weight, tokens.data_ptr(), tokens.element_size(), n, weight.data_ptr(), code,
-              weight.shape[0], weight.shape[1], scale, out.data_ptr())
+        _call('elx_embedding_forward', weight, tokens.data_ptr(), tokens.element_size(), n, weight.data_ptr(), code, vocab,
+              width, scale, out.data_ptr())
     return out
 
 

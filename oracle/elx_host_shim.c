@@ -571,6 +571,9 @@ int elx_moments_pack(const float* exp_avg, const float* exp_avg_sq, int64_t n, v
             s[exps_at(n) + b] = e;
             for (int i = 0; i < len; ++i) s[e0 + i] = code_of(x[e0 + i], e, !k, 0.5);
         }
+        const int64_t end = exps_at(n) + blocks_of(n);
+        if (n) memset(s + n, 0, (size_t)(exps_at(n) - n));
+        memset(s + end, 0, (size_t)(elx_moment_state_bytes(n) - end));
     }
     return ELX_OK;
 }

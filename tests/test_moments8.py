@@ -45,6 +45,8 @@ def test_pack_and_unpack_follow_the_definition(host_backend, n):
     assert sm.numel() == sv.numel() == K.moment_state_bytes(n) == _lib().elx_moment_state_bytes(n)
     assert ref.same_state(sm.numpy(), ref.encode(m.astype(np.float64), True, 0.5), n, True)
     assert ref.same_state(sv.numpy(), ref.encode(v.astype(np.float64), False, 0.5), n, False)
+    end = ref.round_up(n, 16) + (n + 255) // 256
+    assert not any(s.numpy()[a:b].any() for s in (sm, sv) for a, b in ((n, ref.round_up(n, 16)), (end, s.numel())))
     out = torch.empty(n), torch.empty(n)
     K.unpack_moments(sm, sv, *out)
     assert np.array_equal(out[0].numpy(), ref.decode(sm.numpy(), n, True))
