@@ -277,6 +277,7 @@ __global__ void __cluster_dims__(kCluster, 1, 1) __launch_bounds__(kClusterThrea
         for (int j = 0; j < 8; ++j) zero.x[j] = 0;
 #pragma unroll 4
         for (int64_t i = me * kClusterThreads + threadIdx.x; i < whole; i += blocks * kClusterThreads) st256(at + 32 * i, zero);
+        next_may_start();
         if (me == 0 && threadIdx.x < head) zeros[threadIdx.x] = 0;
         if (me == 0 && threadIdx.x < tail) at[32 * whole + threadIdx.x] = 0;
         return;
@@ -362,6 +363,7 @@ __global__ void __cluster_dims__(kCluster, 1, 1) __launch_bounds__(kClusterThrea
         }
         cluster.sync();
     }
+    next_may_start();
     for (int i = threadIdx.x; i < mine; i += kClusterThreads) {
         keys_out[base + i] = keys[from * c + i];
         order_out[base + i] = order[from * c + i];
@@ -387,6 +389,7 @@ __global__ void __launch_bounds__(kEmbedThreads) embed_sum_kernel(const uint32_t
     const int64_t piece = static_cast<int64_t>(blockIdx.x) * blockDim.y + threadIdx.y, first = piece * kPiece;
     uint32_t* const key = s_key[threadIdx.y];
     uint32_t* const pos = s_pos[threadIdx.y];
+    after_previous();
     for (int i = threadIdx.x; i < kPiece + 2; i += blockDim.x) {
         const int64_t at = first + i - 1;
         key[i] = at >= 0 && at < n ? keys[at] : 0xFFFFFFFFu;   // larger than any key
@@ -437,6 +440,7 @@ __global__ void __launch_bounds__(kEmbedThreads) embed_sum_kernel(const uint32_t
             }
         }
     }
+    next_may_start();
 }
 
 // VEC sums of a partial row.
@@ -494,6 +498,7 @@ __global__ void __launch_bounds__(32 * kJoinWarps) embed_join_kernel(const uint3
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int64_t piece0 = static_cast<int64_t>(blockIdx.x) * kJoinWarps;
     if (threadIdx.x == 0) s_long = 0;
+    after_previous();
     __syncthreads();
     const int c = (blockIdx.y * 32 + lane) * VEC;
     uint32_t key = 0;
@@ -588,15 +593,17 @@ int launch_sums(const uint32_t* keys, const uint32_t* order, int64_t n, const vo
     while (block.y > 1 && pieces < 296ll * block.y) block.y /= 2;
     const int slabs = (width / VEC + block.x - 1) / block.x;
     const dim3 grid(static_cast<unsigned>((pieces + block.y - 1) / block.y), static_cast<unsigned>(slabs < 64 ? slabs : 64));
-    embed_sum_kernel<DT, VEC><<<grid, block, 0, s>>>(keys, order, n, dout, static_cast<uint32_t>(vocab), width, scale, dweight, partial);
-    if (pieces > 1) {
+    cudaError_t e = launch_next(embed_sum_kernel<DT, VEC>, grid, block, s, keys, order, n, dout, static_cast<uint32_t>(vocab), width, scale,
+                                dweight, partial);
+    if (e == cudaSuccess && pieces > 1) {
         const int join_slabs = (width / VEC + 31) / 32;
         const dim3 join(static_cast<unsigned>((pieces + kJoinWarps - 1) / kJoinWarps),
                         static_cast<unsigned>(join_slabs < 64 ? join_slabs : 64));
-        embed_join_kernel<DT, VEC><<<join, 32 * kJoinWarps, 0, s>>>(keys, n, static_cast<uint32_t>(vocab), width, scale, dweight,
-                                                                      partial);
+        e = launch_next(embed_join_kernel<DT, VEC>, join, dim3(32 * kJoinWarps), s, keys, n, static_cast<uint32_t>(vocab), width, scale,
+                        dweight, partial);
     }
-    return record_cuda(cudaGetLastError());
+    if (e != cudaSuccess) (void)cudaGetLastError();
+    return record_cuda(e);
 }
 
 // Elements per access: 16 bytes, a word of two 16-bit elements, or one element -- what the width and the addresses allow.

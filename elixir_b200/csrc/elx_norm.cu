@@ -585,6 +585,7 @@ __global__ void __launch_bounds__(512, 1) norm_backward_kernel(const NormArgs a)
             rstd = next_rstd;
         }
     }
+    next_may_start();
     if (!a.partial) return;
     float* const part = a.partial + static_cast<int64_t>(blockIdx.x) * 2 * a.cols;
     for (int g = 0; g < groups; ++g) {
@@ -665,6 +666,7 @@ __global__ void __launch_bounds__(1024) norm_columns_kernel(const float* __restr
     __shared__ float s[2][32][33];
     const int c = blockIdx.x * 32 + threadIdx.x;
     float dw = 0.0f, db = 0.0f;
+    after_previous();
     if (c < cols) {
         for (int g = threadIdx.y; g < groups; g += 32) {
             dw += partial[static_cast<int64_t>(g) * 2 * cols + c];
@@ -836,8 +838,10 @@ int backward_dt(NormArgs& a, bool wide_ok, bool same_mis, void* dweight, void* d
         }
     }
     if (rc != ELX_OK || !a.partial) return rc;
-    norm_columns_kernel<DT><<<(a.cols + 31) / 32, dim3(32, 32), 0, s>>>(a.partial, a.groups, a.cols, dweight, dbias);
-    return record_cuda(cudaGetLastError());
+    const cudaError_t e = launch_next(norm_columns_kernel<DT>, dim3((a.cols + 31) / 32), dim3(32, 32), s, a.partial, a.groups, a.cols,
+                                      dweight, dbias);
+    if (e != cudaSuccess) (void)cudaGetLastError();
+    return record_cuda(e);
 }
 
 // Elements from the last 16-byte boundary to p.
