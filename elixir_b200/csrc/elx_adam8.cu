@@ -215,10 +215,11 @@ __device__ __forceinline__ float2 new_param2(float2 p, float2 m, float2 v, const
 // needs the largest of its new moments, which stay in registers, and one redux instruction per moment gives it.  So no
 // computing warp ever waits for another; each tells the mover by itself that its part of the stage is done.
 //
-// The bytes bound it (16 per element of 16-bit chunks): the arithmetic is held to about 50 instructions per element,
-// of which the issue slots allow 88 at the full HBM rate -- dither bits 9, decoding and encoding 16, Adam 20 -- by
-// folding every scale into one product, keeping codes in the top byte of a word, and leaving all that is rare (huge or
-// non-finite moments, block borders) to update_block().
+// The bytes bound it (16 per element of 16-bit chunks): 8 x 32 Mi elements take 732 us, 5.87 TB/s, against 1253 us and
+// 5.98 TB/s for the update with fp32 moments, and 6.4 TB/s for a plain copy.  The arithmetic takes about 60 instructions per
+// element and so 60 % of the issue slots; packed fp32 operations, scales folded into one product, codes kept in the top byte
+// of a word and all that is rare (huge or non-finite moments, block borders) left to update_block() keep it there.  One
+// launch of three small shards takes 8 us, most of it the first tile's way through the ring.
 struct Adam8Args {
     const ElxChunkDesc* descs;
     const ElxSeg* segs;
@@ -703,7 +704,8 @@ __device__ __forceinline__ void pack_pair(const float* __restrict__ x, uint8_t* 
     if ((lane & 15) == 0) state[moment_exps_at(n) + pair * 2 + (lane >> 4)] = static_cast<uint8_t>(exp);
 }
 
-// Bound by the bytes: 8 in and 2 out per element, 7 of 8 of them in whole lines per warp.
+// Bound by the bytes: 8 in and 2 out per element; 64 Mi elements in 110 us (6.1 TB/s).  Back into fp32: 115 us, into bf16
+// (32 Mi) 36 us.
 __global__ void __launch_bounds__(kConvThreads) pack_kernel(const float* __restrict__ m, const float* __restrict__ v, int64_t n,
                                                             uint8_t* state_m, uint8_t* state_v, int vec) {
     const int64_t pairs = (n + kPair - 1) / kPair, stride = static_cast<int64_t>(gridDim.x) * (kConvThreads / 32);

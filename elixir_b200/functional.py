@@ -3,9 +3,11 @@
 ``ElixirModule(use_fused_kernels=True)`` runs the ``nn.LayerNorm`` and ``nn.Embedding`` layers of its module through
 them (``use_kernels``), where the reference swaps in a fused layer norm (``elixir/kernels/layernorm.py:4``,
 ``elixir/hook/parameter.py:69-70``).  Statistics and sums are fp32, every output is rounded once, and both parameter
-gradients are summed in an order that the inputs alone fix.  CUDA tensors only; first derivatives only.
+gradients are summed in an order that the inputs alone fix.  CUDA tensors only; first derivatives only.  As with every
+autograd function, a backward pass is captured into a CUDA graph only while no eager graph of the same parameters is alive.
 """
 from functools import partial
+from math import prod
 from typing import Optional
 
 import torch
@@ -13,7 +15,7 @@ import torch.nn as nn
 from torch.autograd import Function
 from torch.autograd.function import once_differentiable
 
-from . import kernels
+from . import _abi, kernels
 
 _DTYPES = (torch.float16, torch.bfloat16, torch.float32)
 
@@ -24,6 +26,7 @@ class _LayerNorm(Function):
     def forward(ctx, x, weight, bias, eps):
         y, mean, rstd = kernels.layer_norm_forward(x, weight, bias, eps)
         ctx.save_for_backward(x, weight, mean, rstd)
+        ctx.bias_shape = None if bias is None else bias.shape
         return y
 
     @staticmethod
@@ -33,7 +36,8 @@ class _LayerNorm(Function):
         dx, dweight, dbias = kernels.layer_norm_backward(dy.contiguous(), x, weight, mean, rstd,
                                                          weight_grad=ctx.needs_input_grad[1],
                                                          bias_grad=ctx.needs_input_grad[2])
-        return dx if ctx.needs_input_grad[0] else None, dweight, dbias, None
+        return (dx if ctx.needs_input_grad[0] else None, None if dweight is None else dweight.view(weight.shape),
+                None if dbias is None else dbias.view(ctx.bias_shape), None)
 
 
 def layer_norm(x: torch.Tensor, normalized_shape, weight: Optional[torch.Tensor] = None,
@@ -48,11 +52,8 @@ def layer_norm(x: torch.Tensor, normalized_shape, weight: Optional[torch.Tensor]
     flat = x.contiguous()
     if len(shape) > 1:
         flat = flat.flatten(-len(shape))
-        weight = None if weight is None else weight.contiguous().flatten()
-        bias = None if bias is None else bias.contiguous().flatten()
-    else:
-        weight = None if weight is None else weight.contiguous()
-        bias = None if bias is None else bias.contiguous()
+    # the parameters themselves, not views of them: the memory of a chunk may be another by the time of the backward pass
+    weight, bias = (t if t is None else t.contiguous() for t in (weight, bias))
     return _LayerNorm.apply(flat, weight, bias, eps).view(x.shape)
 
 
@@ -95,7 +96,7 @@ def _plain_cuda(x, *params):
 
 
 def _layer_norm_layer(layer: nn.LayerNorm, x):
-    if x.dtype in _DTYPES and all(p is None or p.dtype == x.dtype for p in (layer.weight, layer.bias)) and _plain_cuda(
+    if x.dtype in _DTYPES and 0 < prod(layer.normalized_shape) <= _abi.NORM_MAX_COLS and all(p is None or p.dtype == x.dtype for p in (layer.weight, layer.bias)) and _plain_cuda(
             x, layer.weight, layer.bias):
         return layer_norm(x, layer.normalized_shape, layer.weight, layer.bias, layer.eps)
     return nn.LayerNorm.forward(layer, x)
@@ -103,7 +104,7 @@ def _layer_norm_layer(layer: nn.LayerNorm, x):
 
 def _embedding_layer(layer: nn.Embedding, tokens):
     if (tokens.dtype in (torch.int32, torch.int64) and layer.max_norm is None and not layer.sparse
-            and not layer.scale_grad_by_freq and _plain_cuda(tokens, layer.weight)):
+            and not layer.scale_grad_by_freq and layer.weight.numel() > 0 and _plain_cuda(tokens, layer.weight)):
         return embedding(tokens, layer.weight, layer.padding_idx)
     return nn.Embedding.forward(layer, tokens)
 

@@ -724,6 +724,8 @@ def pack_moments(exp_avg: torch.Tensor, exp_avg_sq: torch.Tensor, state_m: Optio
             raise ValueError(f'{name} must hold moment_state_bytes({n}) = {size} bytes')
     _same_device(('exp_avg', exp_avg), ('exp_avg_sq', exp_avg_sq), ('state_m', state_m), ('state_v', state_v))
     if n:
+        if state_m.data_ptr() == state_v.data_ptr():
+            raise ValueError('the two state arrays are one')
         _call('elx_moments_pack', exp_avg, exp_avg.data_ptr(), exp_avg_sq.data_ptr(), n, state_m.data_ptr(), state_v.data_ptr())
     return state_m, state_v
 
@@ -738,12 +740,15 @@ def unpack_moments(state_m: torch.Tensor, state_v: torch.Tensor, exp_avg: torch.
     n = exp_avg.numel()
     if exp_avg_sq.numel() != n:
         raise ValueError('the two moments differ in size')
+    size = moment_state_bytes(n)
     for name, t in (('state_m', state_m), ('state_v', state_v)):
         _check_tensor(t, name, torch.uint8)
-        if t.numel() != moment_state_bytes(n):
-            raise ValueError(f'{name} must hold moment_state_bytes({n}) = {moment_state_bytes(n)} bytes')
+        if t.numel() != size:
+            raise ValueError(f'{name} must hold moment_state_bytes({n}) = {size} bytes')
     _same_device(('exp_avg', exp_avg), ('exp_avg_sq', exp_avg_sq), ('state_m', state_m), ('state_v', state_v))
     if n:
+        if exp_avg.data_ptr() == exp_avg_sq.data_ptr():
+            raise ValueError('the two moments are one tensor')
         _call('elx_moments_unpack', exp_avg, state_m.data_ptr(), state_v.data_ptr(), n, dtype_code(exp_avg.dtype),
               exp_avg.data_ptr(), exp_avg_sq.data_ptr())
 

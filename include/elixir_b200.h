@@ -563,7 +563,7 @@ int elx_moments_unpack(const void* state_m, const void* state_v, int64_t n, int 
  * elx_layer_norm_backward: dx, and the sums over the rows dweight = sum dy xhat and dbias = sum dy (each `cols`
  * elements, NULL = not wanted), in an order that depends on rows and cols alone.  The sums need a workspace of
  * elx_layer_norm_backward_workspace(rows, cols) bytes, 16-byte aligned, not shared with a call that may run at the
- * same time; without them it may be NULL.  dx must not overlap the inputs.
+ * same time; without them it may be NULL.  y and dx must not overlap the inputs.
  */
 #define ELX_NORM_MAX_COLS 1048576
 int elx_layer_norm_forward(const void* x, const void* weight, const void* bias, int dtype, int64_t rows, int64_t cols,

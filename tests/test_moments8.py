@@ -221,6 +221,10 @@ def test_refusals(host_backend):
         K.pack_moments(x, y, s[:-1], s)
     with pytest.raises(ValueError):
         K.pack_moments(torch.zeros(2 * n)[::2], y)    # not contiguous
+    with pytest.raises(ValueError):
+        K.pack_moments(x, y, s, s)
+    with pytest.raises(ValueError):
+        K.unpack_moments(s, s, x, x)
     with pytest.raises(TypeError):
         K.unpack_moments(s, s, x.half(), y.half())
     with pytest.raises(TypeError):

@@ -260,6 +260,23 @@ def test_autograd(cuda, shape, norm):
         assert abs(slope - want) <= 0.02 * (1 + float((got[k].double() * direction).abs().sum()))
 
 
+@pytest.mark.parametrize('norm', [(40, ), (5, 8)])
+def test_parameters_whose_memory_moves_before_the_backward_pass(cuda, norm):
+    """As with the chunks of a small replica cache: the gradient is that of the values in the parameter's new memory."""
+    from elixir_b200 import functional as F
+    gen = torch.Generator(device=cuda).manual_seed(3)
+    x = torch.randn((6, ) + norm, generator=gen, device=cuda).requires_grad_()
+    dy = torch.randn((6, ) + norm, generator=gen, device=cuda)
+    w, b = (torch.nn.Parameter(torch.randn(norm, generator=gen, device=cuda)) for _ in range(2))
+    want = torch.autograd.grad(F.layer_norm(x, norm, w, b), (x, w, b), dy)
+    y = F.layer_norm(x, norm, w, b)
+    old = w.data
+    w.data = old.clone()
+    old.fill_(float('nan'))
+    got = torch.autograd.grad(y, (x, w, b), dy)
+    assert all(torch.equal(g, e) and g.shape == e.shape for g, e in zip(got, want))
+
+
 def test_autograd_forms(cuda):
     from elixir_b200 import functional as F
     x = torch.randn(6, 32, device=cuda)
