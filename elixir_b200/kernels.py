@@ -715,9 +715,9 @@ def pack_moments(exp_avg: torch.Tensor, exp_avg_sq: torch.Tensor, state_m: Optio
         raise ValueError('the two moments differ in size')
     size = moment_state_bytes(n)
     if state_m is None:
-        state_m = torch.empty(size, dtype=torch.uint8, device=exp_avg.device)
+        state_m = exp_avg.new_empty(size, dtype=torch.uint8)
     if state_v is None:
-        state_v = torch.empty(size, dtype=torch.uint8, device=exp_avg.device)
+        state_v = exp_avg.new_empty(size, dtype=torch.uint8)
     for name, t in (('state_m', state_m), ('state_v', state_v)):
         _check_tensor(t, name, torch.uint8)
         if t.numel() != size:
@@ -802,12 +802,12 @@ def layer_norm_backward(dy: torch.Tensor, x: torch.Tensor, weight: Optional[torc
             raise ValueError(f'{name} must have one element per row')
     _same_device(('x', x), ('dy', dy), ('mean', mean), ('rstd', rstd))
     dx = torch.empty_like(x)
-    dweight = torch.empty(cols, dtype=x.dtype, device=x.device) if weight_grad and weight is not None else None
-    dbias = torch.empty(cols, dtype=x.dtype, device=x.device) if bias_grad else None
+    dweight = x.new_empty(cols) if weight_grad and weight is not None else None
+    dbias = x.new_empty(cols) if bias_grad else None
     space, size = None, 0
     if dweight is not None or dbias is not None:
         size = _lib.get().elx_layer_norm_backward_workspace(rows, cols)
-        space = torch.empty(size, dtype=torch.uint8, device=x.device)
+        space = x.new_empty(size, dtype=torch.uint8)
     _call('elx_layer_norm_backward', x, dy.data_ptr(), x.data_ptr(), _addr(weight), mean.data_ptr(), rstd.data_ptr(),
           dtype_code(x.dtype), rows, cols, dx.data_ptr(), _addr(dweight), _addr(dbias), _addr(space), size)
     return dx, dweight, dbias
@@ -849,9 +849,9 @@ def embedding_backward(tokens: torch.Tensor, dout: torch.Tensor, vocab: int, sca
         raise ValueError('padding_idx outside the table')
     _same_device(('dout', dout), ('tokens', tokens))
     code, width, n = dtype_code(dout.dtype), dout.shape[-1], tokens.numel()
-    dweight = torch.empty((vocab, width), dtype=dout.dtype, device=dout.device)
+    dweight = dout.new_empty((vocab, width))
     size = _lib.get().elx_embedding_backward_workspace(n, width)
-    space = torch.empty(size, dtype=torch.uint8, device=dout.device)
+    space = dout.new_empty(size, dtype=torch.uint8)
     _call('elx_embedding_backward', dout, tokens.data_ptr(), tokens.element_size(), n, dout.data_ptr(), code, vocab, width, scale,
           -1 if padding_idx is None else padding_idx, dweight.data_ptr(), space.data_ptr(), size)
     return dweight
