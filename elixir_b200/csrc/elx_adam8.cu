@@ -765,9 +765,23 @@ __global__ void __launch_bounds__(kConvThreads) unpack_kernel(const uint8_t* __r
             unpack_codes<FirstMoment, DT>(cm, sm, om + e);
             unpack_codes<SecondMoment, DT>(cv, sv, ov + e);
         } else {
-            for (int64_t i = q * kPair + lane; i < min((q + 1) * kPair, n); i += 32) {
-                om[i] = Lp<DT>::from_float(decode<FirstMoment>(state_m[i], decode_scale(exps_m[i / kMomentBlock])));
-                ov[i] = Lp<DT>::from_float(decode<SecondMoment>(state_v[i], decode_scale(exps_v[i / kMomentBlock])));
+            // element by element: the codes of one moment after the other, all on their way before the first is decoded
+            const int64_t first = q * kPair + lane;
+            const uint8_t* const codes[2] = {state_m, state_v};
+#pragma unroll
+            for (int k = 0; k < 2; ++k) {
+                uint32_t c[16];
+                float scale[2];
+#pragma unroll
+                for (int j = 0; j < 2; ++j)
+                    scale[j] = q * kPair + j * kMomentBlock < n ? decode_scale((k ? exps_v : exps_m)[2 * q + j]) : 0.0f;
+#pragma unroll
+                for (int j = 0; j < 16; ++j) c[j] = first + 32 * j < n ? codes[k][first + 32 * j] : 0u;
+#pragma unroll
+                for (int j = 0; j < 16; ++j)
+                    if (first + 32 * j < n)
+                        (k ? ov : om)[first + 32 * j] = Lp<DT>::from_float(k ? decode<SecondMoment>(c[j], scale[j / 8])
+                                                                              : decode<FirstMoment>(c[j], scale[j / 8]));
             }
         }
     }
