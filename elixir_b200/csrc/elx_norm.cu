@@ -429,10 +429,14 @@ __global__ void __launch_bounds__(1024) norm_forward_wide_kernel(const NormArgs 
 // With norm_columns_kernel, fp16: 8192 x 1600 23.5 us (3.3 TB/s), 16384 x 2048 41.8 us (4.8 TB/s), 16384 x 4096 78 us
 // (5.2 TB/s); bound by what a row waits for: its loads, one barrier, its sums.  Rows of more than 1024 pieces (NEXT off) lose
 // what is not on its way early: 4096 x 9216 113 us (2.0 TB/s).
+// VPL 1 up to 96 pieces: 32768 x 768 fp16 37 us against 39 with two per thread, 65536 x 256 28.6 us against 31.4 in 512 threads;
+// wider rows lose more by another warp's part of each row's sums (16384 x 1600 40 us with two per thread, 47 with one, 42 with
+// three).
+constexpr int backward_threads(int vpl) { return vpl == 1 ? 768 : 512; }
 template <int DT, int VEC, int VPL, bool NEXT, bool ODD>
-__global__ void __launch_bounds__(512, 1) norm_backward_kernel(const NormArgs a) {
+__global__ void __launch_bounds__(backward_threads(VPL), 1) norm_backward_kernel(const NormArgs a) {
     extern __shared__ float s_cols[];                 // 2 x cols, where there are several groups
-    __shared__ float2 s_sum[2][16][16];               // [row parity][group][warp]
+    __shared__ float2 s_sum[2][24][16];               // [row parity][group][warp]
     const int threads = a.group_threads, group = threadIdx.x / threads, t = threadIdx.x - group * threads;
     const int groups = blockDim.x / threads, warps = threads >> 5, warp = t >> 5;
     using V = Values<VEC>;
@@ -803,7 +807,7 @@ template <int DT, int VEC, int VPL, bool NEXT, bool ODD>
 int launch_backward(NormArgs& a, cudaStream_t s) {
     const int pieces = ODD ? (a.cols + 2 * VEC - 2) / VEC : (a.cols + VEC - 1) / VEC;
     a.group_threads = round32((pieces + VPL - 1) / VPL);
-    int per_block = 512 / a.group_threads;
+    int per_block = backward_threads(VPL) / a.group_threads;
     if (per_block > 15 && a.group_threads > 32) per_block = 15;   // named barriers
     while (per_block > 1 && a.rows < 148 * (per_block - 1)) --per_block;   // few rows: more blocks rather than fuller ones
     a.groups = row_blocks((a.rows + per_block - 1) / per_block, per_block, ODD ? VEC : 1);
@@ -819,12 +823,12 @@ int backward_dt(NormArgs& a, bool wide_ok, bool same_mis, void* dweight, void* d
     int rc = 1;
     if (wide_ok) {
         const int vecs = a.cols / V;
-        if (vecs <= 32) rc = launch_backward<DT, V, 1, true, false>(a, s);
+        if (vecs <= 96) rc = launch_backward<DT, V, 1, true, false>(a, s);
         else if (vecs <= 1024) rc = launch_backward<DT, V, 2, true, false>(a, s);
         else if (vecs <= 2048) rc = launch_backward<DT, V, 4, false, false>(a, s);
     } else if (same_mis && a.cols >= 4 * V) {
         const int pieces = (a.cols + 2 * V - 2) / V;
-        if (pieces <= 32) rc = launch_backward<DT, V, 1, true, true>(a, s);
+        if (pieces <= 96) rc = launch_backward<DT, V, 1, true, true>(a, s);
         else if (pieces <= 1024) rc = launch_backward<DT, V, 2, true, true>(a, s);
         else if (pieces <= 2048) rc = launch_backward<DT, V, 4, false, true>(a, s);
     } else {
