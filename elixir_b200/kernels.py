@@ -389,6 +389,8 @@ class ChunkTable:
         n_moment = n if self.state_bits == 32 else moment_state_bytes(n)
         if not (exp_avg.numel() == exp_avg_sq.numel() == n_moment and grad_param.numel() == n):
             raise ValueError('master, moments and the low-precision shard differ in size')
+        if self.state_bits == 8 and n and exp_avg.data_ptr() == exp_avg_sq.data_ptr():
+            raise ValueError('the two state arrays are one')
         if not 0 <= n_valid <= n:
             raise ValueError('n_valid outside [0, n_shard]')
         if grad_src is not None:

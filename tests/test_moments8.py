@@ -194,6 +194,8 @@ def test_refusals(host_backend):
         table.add_chunk(p, torch.zeros(n), torch.zeros(n), g, n)    # fp32 moments in an 8-bit table
     with pytest.raises(ValueError):
         table.add_chunk(p, s[:-1], s, g, n)
+    with pytest.raises(ValueError):
+        table.add_chunk(p, s, s, g, n, [(0, n, 0)])    # one array for both
     table.add_chunk(p, s, s.clone(), g, n, [(0, n, 0)])
     table.finalize().set_hyper([K.hyper()])
     with pytest.raises(TypeError):
