@@ -49,8 +49,10 @@ def _ptr(t: Optional[torch.Tensor]):
 
 
 try:    # the handle without a Stream object around it: 0.1 us instead of 2.5 us of every call
-    from torch._C import _cuda_getCurrentRawStream as _raw_stream
+    from torch._C import _cuda_getCurrentRawStream as _raw_stream, _cuda_getDevice as _current_device
 except ImportError:
+    _current_device = torch.cuda.current_device
+
     def _raw_stream(index):
         return torch.cuda.current_stream(index).cuda_stream
 
@@ -66,7 +68,7 @@ def _call(name: str, home: torch.Tensor, *args):
     entry, index = getattr(_lib.get(), name), home.get_device()
     if index < 0:    # host-memory backend
         status = entry(*args, None)
-    elif index == torch.cuda.current_device():
+    elif index == _current_device():
         status = entry(*args, _raw_stream(index))
     else:
         with torch.cuda.device(index):
@@ -695,11 +697,11 @@ def moment_state_bytes(n: int) -> int:
     return (n + 15) // 16 * 16 + ((n + _abi.MOMENT_BLOCK - 1) // _abi.MOMENT_BLOCK + 15) // 16 * 16
 
 
-def _same_device(*named):
-    index = named[0][1].get_device()
-    for name, t in named:
+def _same_device(home, *others):
+    index = home.get_device()
+    for t in others:
         if t is not None and t.get_device() != index:
-            raise ValueError(f'{name} is on {t.device}, {named[0][0]} on {named[0][1].device}')
+            raise ValueError(f'tensors on {t.device} and on {home.device}')
 
 
 def _addr(t: Optional[torch.Tensor]):
@@ -724,7 +726,7 @@ def pack_moments(exp_avg: torch.Tensor, exp_avg_sq: torch.Tensor, state_m: Optio
         _check_tensor(t, name, torch.uint8)
         if t.numel() != size:
             raise ValueError(f'{name} must hold moment_state_bytes({n}) = {size} bytes')
-    _same_device(('exp_avg', exp_avg), ('exp_avg_sq', exp_avg_sq), ('state_m', state_m), ('state_v', state_v))
+    _same_device(exp_avg, exp_avg_sq, state_m, state_v)
     if n:
         if state_m.data_ptr() == state_v.data_ptr():
             raise ValueError('the two state arrays are one')
@@ -747,7 +749,7 @@ def unpack_moments(state_m: torch.Tensor, state_v: torch.Tensor, exp_avg: torch.
         _check_tensor(t, name, torch.uint8)
         if t.numel() != size:
             raise ValueError(f'{name} must hold moment_state_bytes({n}) = {size} bytes')
-    _same_device(('exp_avg', exp_avg), ('exp_avg_sq', exp_avg_sq), ('state_m', state_m), ('state_v', state_v))
+    _same_device(exp_avg, exp_avg_sq, state_m, state_v)
     if n:
         if exp_avg.data_ptr() == exp_avg_sq.data_ptr():
             raise ValueError('the two moments are one tensor')
@@ -762,9 +764,9 @@ def unpack_moments(state_m: torch.Tensor, state_v: torch.Tensor, exp_avg: torch.
 
 def _check_norm(x, weight, bias):
     _check_tensor(x, 'x')
-    if x.dim() < 1 or x.shape[-1] < 1:
+    cols = x.shape[-1] if x.dim() else 0
+    if cols < 1:
         raise ValueError('x needs a last dimension of at least one element')
-    cols = x.shape[-1]
     if cols > _abi.NORM_MAX_COLS:
         raise ValueError(f'at most {_abi.NORM_MAX_COLS} elements per row are supported')
     for name, t in (('weight', weight), ('bias', bias)):
@@ -772,7 +774,7 @@ def _check_norm(x, weight, bias):
             _check_tensor(t, name, x.dtype)
             if t.numel() != cols:
                 raise ValueError(f'{name} must have {cols} elements')
-    _same_device(('x', x), ('weight', weight), ('bias', bias))
+    _same_device(x, weight, bias)
     return x.numel() // cols, cols
 
 
@@ -802,7 +804,7 @@ def layer_norm_backward(dy: torch.Tensor, x: torch.Tensor, weight: Optional[torc
         _check_tensor(t, name, torch.float32)
         if t.numel() != rows:
             raise ValueError(f'{name} must have one element per row')
-    _same_device(('x', x), ('dy', dy), ('mean', mean), ('rstd', rstd))
+    _same_device(x, dy, mean, rstd)
     dx = torch.empty_like(x)
     dweight = x.new_empty(cols) if weight_grad and weight is not None else None
     dbias = x.new_empty(cols) if bias_grad else None
@@ -828,7 +830,7 @@ def embedding_forward(tokens: torch.Tensor, weight: torch.Tensor, scale: float =
     _check_tensor(weight, 'weight')
     if weight.dim() != 2 or weight.numel() == 0:
         raise ValueError('weight must be a table of at least one row and one column')
-    _same_device(('weight', weight), ('tokens', tokens))
+    _same_device(weight, tokens)
     code, (vocab, width), n = dtype_code(weight.dtype), weight.shape, tokens.numel()
     out = weight.new_empty((*tokens.shape, width))
     if n:
@@ -849,7 +851,7 @@ def embedding_backward(tokens: torch.Tensor, dout: torch.Tensor, vocab: int, sca
         raise ValueError('the table needs at least one row')
     if padding_idx is not None and not 0 <= padding_idx < vocab:
         raise ValueError('padding_idx outside the table')
-    _same_device(('dout', dout), ('tokens', tokens))
+    _same_device(dout, tokens)
     code, width, n = dtype_code(dout.dtype), dout.shape[-1], tokens.numel()
     dweight = dout.new_empty((vocab, width))
     size = _lib.get().elx_embedding_backward_workspace(n, width)
