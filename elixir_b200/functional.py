@@ -95,29 +95,36 @@ def _plain_cuda(x, *params):
             and not torch.is_autocast_enabled('cuda') and not torch._C._are_functorch_transforms_active())
 
 
+# torch's own, as they were when this module was imported: a class that has been given another one keeps that
+_TORCH_FORWARD = {kind: kind.forward for kind in (nn.LayerNorm, nn.Embedding)}
+
+
 def _layer_norm_layer(layer: nn.LayerNorm, x):
-    if x.dtype in _DTYPES and 0 < prod(layer.normalized_shape) <= _abi.NORM_MAX_COLS and all(p is None or p.dtype == x.dtype for p in (layer.weight, layer.bias)) and _plain_cuda(
+    if type(layer).forward is _TORCH_FORWARD[nn.LayerNorm] and x.dtype in _DTYPES and 0 < prod(layer.normalized_shape) <= _abi.NORM_MAX_COLS and all(p is None or p.dtype == x.dtype for p in (layer.weight, layer.bias)) and _plain_cuda(
             x, layer.weight, layer.bias):
         return layer_norm(x, layer.normalized_shape, layer.weight, layer.bias, layer.eps)
-    return nn.LayerNorm.forward(layer, x)
+    return type(layer).forward(layer, x)
 
 
 def _embedding_layer(layer: nn.Embedding, tokens):
-    if (tokens.dtype in (torch.int32, torch.int64) and layer.max_norm is None and not layer.sparse
+    if (type(layer).forward is _TORCH_FORWARD[nn.Embedding] and tokens.dtype in (torch.int32, torch.int64) and layer.max_norm is None and not layer.sparse
             and not layer.scale_grad_by_freq and layer.weight.numel() > 0 and _plain_cuda(tokens, layer.weight)):
         return embedding(tokens, layer.weight, layer.padding_idx)
-    return nn.Embedding.forward(layer, tokens)
+    return type(layer).forward(layer, tokens)
 
 
 def use_kernels(module: nn.Module) -> int:
     """Run every ``nn.LayerNorm`` and ``nn.Embedding`` of ``module`` (subclasses that keep their ``forward`` included)
     through this package's kernels wherever those apply: CUDA tensors, one type for input and parameters, no autocast;
-    embeddings without ``max_norm``, ``sparse`` and ``scale_grad_by_freq``.  Other calls stay with torch.  Returns the
-    number of layers."""
+    embeddings without ``max_norm``, ``sparse`` and ``scale_grad_by_freq``.  Other calls stay with torch.  A layer with a
+    ``forward`` of its own, set on the layer or on its class, keeps that.  Returns the number of layers."""
     count = 0
     for layer in module.modules():
         for kind, forward in ((nn.LayerNorm, _layer_norm_layer), (nn.Embedding, _embedding_layer)):
-            if isinstance(layer, kind) and type(layer).forward is kind.forward:
+            if not isinstance(layer, kind) or type(layer).forward is not _TORCH_FORWARD[kind]:
+                continue
+            own = layer.__dict__.get('forward')    # None, or what a call before this one put there
+            if own is None or (isinstance(own, partial) and own.func is forward):
                 layer.forward = partial(forward, layer)
                 count += 1
     return count

@@ -113,3 +113,33 @@ def test_layers_of_a_module(monkeypatch):
         twin[1].weight.fill_(3.0)
     assert not torch.equal(twin[1](x), model[1](x)) and torch.equal(want[1], model[1](x))
     assert list(twin.state_dict()) == list(model.state_dict())
+
+
+def test_a_layer_keeps_a_forward_of_its_own():
+    """Set on the layer, before or after the layers change hands, or on the class by a program that patches torch."""
+    from elixir_b200 import functional as F
+    tokens, x = torch.tensor([[1, 2], [3, 9]]), torch.randn(3, 8)
+    model = nn.Sequential(nn.Embedding(10, 8), nn.LayerNorm(8), nn.LayerNorm(8))
+    want = [2 * model[0](tokens), 2 * model[1](x), model[2](x)]
+    for layer in model[:2]:
+        layer.forward = lambda t, own=layer.forward: 2 * own(t)
+    own = [layer.__dict__['forward'] for layer in model[:2]]
+    for _ in range(2):
+        assert F.use_kernels(model) == 1
+        assert [layer.__dict__['forward'] for layer in model[:2]] == own
+        assert all(torch.equal(w, layer(t)) for w, layer, t in zip(want, model, (tokens, x, x)))
+    model[2].forward = lambda t, own=model[2].forward: 3 * own(t)    # around the one that use_kernels put there
+    assert F.use_kernels(model) == 0 and torch.equal(model[2](x), 3 * want[2])
+
+
+@pytest.mark.parametrize('kind,shape', [(nn.LayerNorm, (8, )), (nn.Embedding, (10, 8))])
+def test_a_class_keeps_a_forward_that_it_was_given(monkeypatch, kind, shape):
+    from elixir_b200 import functional as F
+    t = torch.randn(3, 8) if kind is nn.LayerNorm else torch.tensor([[1, 2], [3, 9]])
+    early, late = kind(*shape), kind(*shape)
+    assert F.use_kernels(early) == 1
+    want, torch_forward = 2 * early(t), kind.forward
+    monkeypatch.setattr(kind, 'forward', lambda layer, t: 2 * torch_forward(layer, t))
+    assert F.use_kernels(late) == 0 and 'forward' not in late.__dict__
+    monkeypatch.setattr(F, '_plain_cuda', lambda *a: True)    # as with CUDA tensors: the patch comes first all the same
+    assert torch.equal(early(t), want)
