@@ -293,7 +293,7 @@ class ElixirOptimizer:
     def state_dict(self):
         """This rank's flat optimizer state: one (exp_avg, exp_avg_sq) pair per chunk shard plus the control
         block fields.  The reference saves none of this (its scaler state is lost on restart).  8-bit moments are
-        saved as they are held; ``load_state_dict`` takes moments saved in either form."""
+        saved as they are held; ``load_state_dict`` takes moments saved in either form, numbers of any floating type."""
         self._quiesce_host_shards()
         self.engine.check_status()
         if not self.scaled_optimizer:
@@ -311,13 +311,14 @@ class ElixirOptimizer:
             torch.cuda.synchronize(self.engine.device)
 
     def _load_moments(self, shard, exp_avg, exp_avg_sq):
-        """Moments saved in either form into this optimizer's form."""
-        if exp_avg.dtype == shard[1].dtype:
+        """Moments saved in either form, as numbers of any type or as 8-bit states, into this optimizer's form."""
+        packed = torch.uint8 in (exp_avg.dtype, exp_avg_sq.dtype)
+        if packed == (self.engine.state_bits == 8):
             shard[1].copy_(exp_avg)
             shard[2].copy_(exp_avg_sq)
-        elif self.engine.state_bits == 8:
-            device = shard[1].device
-            kernels.pack_moments(exp_avg.to(device), exp_avg_sq.to(device), shard[1], shard[2])
+        elif not packed:
+            numbers = [t.to(shard[1].device, torch.float32).contiguous() for t in (exp_avg, exp_avg_sq)]
+            kernels.pack_moments(*numbers, shard[1], shard[2])
         elif shard[1].device == self.engine.device:
             device = shard[1].device
             kernels.unpack_moments(exp_avg.to(device), exp_avg_sq.to(device), shard[1], shard[2])

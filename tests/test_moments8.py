@@ -162,6 +162,31 @@ def test_checkpoints_move_between_both_forms(host_backend, saved_bits, loaded_bi
     assert oopt.engine.read_control().step == 2
 
 
+@pytest.mark.parametrize('dtype', [torch.bfloat16, torch.float16, torch.float64])
+@pytest.mark.parametrize('loaded_bits', [8, 32])
+@pytest.mark.parametrize('strided', [False, True])
+def test_checkpoints_hold_moments_of_any_floating_type(host_backend, loaded_bits, dtype, strided):
+    """As a checkpoint that was thinned out has them, and as ``engine.moments(i, torch.bfloat16)`` hands them out."""
+    emodel, eopt = _wrapped(8)
+    for step in range(2):
+        emodel.inject_gradients(_grads(emodel, step))
+        eopt.step()
+    saved = eopt.state_dict()
+    for c, entry in enumerate(saved['shards']):
+        m, v = eopt.engine.moments(c, torch.bfloat16 if dtype is torch.bfloat16 else torch.float32)
+        entry.update(exp_avg=m.to(dtype), exp_avg_sq=v.to(dtype))
+        if strided:
+            entry.update((k, t.repeat_interleave(2)[::2]) for k, t in list(entry.items()))
+    _, oopt = _wrapped(loaded_bits)
+    oopt.load_state_dict(saved)
+    for c, entry in enumerate(saved['shards']):
+        for theirs, key, signed in zip(oopt.engine.moments(c), ('exp_avg', 'exp_avg_sq'), (True, False)):
+            want = entry[key].float().numpy().astype(np.float64)
+            if loaded_bits == 8:
+                want = ref.decode(ref.encode(want, signed, 0.5), want.size, signed)
+            assert np.array_equal(theirs.numpy(), want)
+
+
 def test_engine_step_from_zero_moments_and_sizes_of_one(host_backend):
     from elixir_b200 import kernels as K
     from elixir_b200.engine import ChunkStepEngine
