@@ -149,6 +149,9 @@ __device__ __noinline__ void update_block(const BlockAt& b, const Group8* s_grou
     }
     const uint32_t em = block_exponent(__reduce_max_sync(0xFFFFFFFFu, top_m));
     const uint32_t ev = block_exponent(__reduce_max_sync(0xFFFFFFFFu, top_v));
+    // A block that is not finite, whatever made it so: a finite gradient whose square passes fp32's range does, and so does a
+    // block that was not before.  All 256 elements of it are lost, which is reported like a gradient that is not finite.
+    if (max(em, ev) == 255u) nan_acc = __uint_as_float(0x7FC00000u);
     const float xm = encode_scale(em), xv = encode_scale(ev);
     const bool easy = em <= kEasyM && ev <= kEasyV;
 #pragma unroll

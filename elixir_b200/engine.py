@@ -975,6 +975,6 @@ class ChunkStepEngine:
         c = self.ctl.read()
         if c.status:
             raise RuntimeError(f'elixir_b200 kernels reported status {c.status:#x} '
-                               '(1: non-finite gradient met on an applied step, 2: descriptor table mismatch, '
+                               '(1: non-finite gradient, or block of 8-bit moments, met on an applied step, 2: descriptor table mismatch, '
                                '4: a bounded wait on a copy or on another rank expired; '
                                f'{c.forced_skips} step(s) were skipped because of it)')

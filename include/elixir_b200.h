@@ -47,7 +47,8 @@ extern "C" {
 #define ELX_ERR_CAPACITY (-8)  /* request exceeds a documented fixed capacity                   */
 
 /* sticky bits in ElxCtl.status */
-#define ELX_STAT_LATE_INF 1u   /* the Adam kernel met a non-finite gradient the probe had not flagged */
+#define ELX_STAT_LATE_INF 1u   /* the Adam kernel met a non-finite gradient the probe had not flagged,
+                                  or left a block of 8-bit moments that is not finite */
 #define ELX_STAT_BAD_DESC 2u   /* a kernel could not map a tile to a chunk descriptor                   */
 #define ELX_STAT_TIMEOUT 4u    /* a bounded wait (on-chip barrier or another rank) expired; the kernel gave up.
                                   While the bit is set elx_step_begin decides "skip" and leaves the loss
@@ -70,7 +71,7 @@ typedef struct ElxCtl {
     float    inv_div;          /* 1/div_scale when that product is exact (power of two), else 0   */
     uint32_t skipped_steps;    /* total skipped steps                                             */
     uint32_t status;           /* sticky ELX_STAT_* bits                                          */
-    uint32_t late_inf;         /* set by the Adam kernel when it meets inf/nan on an applied step */
+    uint32_t late_inf;         /* set by the Adam kernel with ELX_STAT_LATE_INF                 */
     uint32_t forced_skips;     /* steps skipped because ELX_STAT_TIMEOUT was set, not for an overflow */
     float    clip_coef;        /* clip factor of the last applied step (1 = not clipped)          */
     float    grad_norm;        /* unscaled global gradient norm of the last applied step          */
@@ -535,7 +536,10 @@ int64_t elx_moment_state_bytes(int64_t n);
  * the expected value of a stored moment is the moment itself.  A second moment above zero is never stored as zero.
  * In a block of which only a part lies inside segments the other elements keep the values of their moments (re-coded
  * where the block's exponent changes); a block outside all segments is left as it is.  A skipped step refreshes the
- * working copies only.  Root and division of the parameter's step are approximate (within 1e-6 relative); "math_mode"
+ * working copies only.  An inf or a NaN costs its whole block: where a gradient is not finite, or a finite one's square
+ * passes fp32's range (|g| above about 5.8e20 after unscaling, with beta2 = 0.999), the block's exponent becomes 255, all
+ * 256 elements of that moment read as NaN and the next update makes their parameters NaN.  ELX_STAT_LATE_INF and late_inf
+ * are raised by every update that leaves such a block.  Root and division of the parameter's step are approximate (within 1e-6 relative); "math_mode"
  * does not apply.  All pointers of a descriptor should be 32-byte aligned; other alignments are handled element by
  * element.
  */

@@ -482,7 +482,7 @@ static uint32_t mix(uint32_t x) {
 }
 
 static void adam8_shard(const ElxChunkDesc* d, int index, const ElxSeg* segs, const ElxHyper* hyper, int n_groups,
-                        const ElxCtl* ctl) {
+                        ElxCtl* ctl) {
     uint8_t *sm = (uint8_t*)d->exp_avg, *sv = (uint8_t*)d->exp_avg_sq;
     uint8_t *em = sm + exps_at(d->n_shard), *ev = sv + exps_at(d->n_shard);
     for (int64_t b = 0; b < blocks_of(d->n_shard) && !ctl->skip; ++b) {
@@ -530,6 +530,10 @@ static void adam8_shard(const ElxChunkDesc* d, int index, const ElxSeg* segs, co
         if (!touched) continue;
         em[b] = block_exp(m, len);
         ev[b] = block_exp(v, len);
+        if (em[b] == 255 || ev[b] == 255) {
+            ctl->late_inf = 1;
+            ctl->status |= ELX_STAT_LATE_INF;
+        }
         uint32_t key = mix((uint32_t)ctl->step * 0x632BE5ABu + (uint32_t)index * 0x9E3779B1u + 0x2545F491u);
         key = mix(mix(key ^ (uint32_t)b) ^ (uint32_t)((uint64_t)b >> 32));
         for (int i = 0; i < len; ++i) {

@@ -167,6 +167,32 @@ def test_a_non_finite_gradient_nobody_probed_is_reported_and_poisons_its_block_o
     assert nan[300] and int(nan.sum()) == 1
 
 
+@pytest.mark.parametrize('dtype', [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize('n', [600, 8192])    # the end of a shard, whole tiles
+def test_a_block_that_is_not_finite_is_reported(cuda, dtype, n):
+    """A finite gradient whose square passes fp32's range costs the second moments of its block, and the control block says
+    so; so it does where the block was lost before."""
+    from elixir_b200 import _abi
+    bad = torch.arange(n, device=cuda) // 256 == 1
+    case = Case(cuda, dtype, [n], [[(0, n, 0)]], [_hyper()], seed=15)
+    case.eng.shards[0][3][300] = 1e21
+    case.eng.probe()
+    case.eng.step()
+    ctl = case.eng.read_control()
+    assert ctl.skip == 0 and ctl.late_inf == 1 and ctl.status == _abi.STAT_LATE_INF
+    m, v = case.eng.moments(0)
+    assert torch.equal(torch.isnan(v), bad) and bool(torch.isfinite(m).all())
+    assert bool(torch.isfinite(case.eng.shards[0][0]).all())    # as with fp32 moments: the element itself hardly moves
+    for which in (1, 2):
+        case = Case(cuda, dtype, [n], [[(0, n, 0)]], [_hyper()], seed=16)
+        case.eng.shards[0][which][ref.round_up(n, 16) + 1] = 255
+        case.eng.probe()
+        case.eng.step()
+        ctl = case.eng.read_control()
+        assert ctl.skip == 0 and ctl.late_inf == 1 and ctl.status == _abi.STAT_LATE_INF
+        assert torch.equal(torch.isnan(case.eng.moments(0)[which - 1]), bad) and torch.equal(torch.isnan(case.eng.shards[0][0]), bad)
+
+
 def test_clipping_divides_by_the_clipped_scale(cuda):
     """With max_norm the divisor is a number the device forms: the restatement takes it from the control block."""
     from elixir_b200.engine import ChunkStepEngine

@@ -202,6 +202,29 @@ def test_engine_step_from_zero_moments_and_sizes_of_one(host_backend):
     assert eng.moments(0)[0].item() in (0.046875, 0.05078125)    # 0.05 is held as one of its neighbours (1 + t/8) 2^-5
 
 
+def test_a_block_that_is_not_finite_is_reported(host_backend):
+    """A finite gradient whose square passes fp32's range, and a block that was lost before."""
+    from elixir_b200 import _abi, kernels as K
+    from elixir_b200.engine import ChunkStepEngine
+    for lost in (False, True):
+        eng = ChunkStepEngine('cpu', torch.bfloat16, state_bits=8)
+        grad = torch.full((600, ), 0.5, dtype=torch.bfloat16)
+        grad[300] = 0.5 if lost else 1e21
+        eng.add_shard(torch.ones(600), grad, 600, [(0, 600, 0)])
+        if lost:
+            eng.shards[0][2][ref.round_up(600, 16) + 1] = 255
+        eng.finalize()
+        eng.set_hyper([K.hyper()])
+        eng.probe()
+        eng.step()
+        ctl = eng.read_control()
+        assert ctl.skip == 0 and ctl.late_inf == 1 and ctl.status == _abi.STAT_LATE_INF
+        m, v = eng.moments(0)
+        assert torch.equal(torch.isnan(v), (torch.arange(600) // 256) == 1) and bool(torch.isfinite(m).all())
+        with pytest.raises(RuntimeError, match='8-bit moments'):
+            eng.check_status()
+
+
 def test_refusals(host_backend):
     from elixir_b200 import _abi, kernels as K
     from elixir_b200.engine import ChunkStepEngine
