@@ -3,8 +3,10 @@
 ``ElixirModule(use_fused_kernels=True)`` runs the ``nn.LayerNorm`` and ``nn.Embedding`` layers of its module through
 them (``use_kernels``), where the reference swaps in a fused layer norm (``elixir/kernels/layernorm.py:4``,
 ``elixir/hook/parameter.py:69-70``).  Statistics and sums are fp32, every output is rounded once, and both parameter
-gradients are summed in an order that the inputs alone fix.  CUDA tensors only; first derivatives only.  As with every
-autograd function, a backward pass is captured into a CUDA graph only while no eager graph of the same parameters is alive.
+gradients are summed in an order that the inputs alone fix.  CUDA tensors only.  ``layer_norm`` and ``embedding`` have first
+derivatives in reverse mode only; forward-mode derivatives of a module's layers stay with torch (``use_kernels``).  As with
+every autograd function, a backward pass is captured into a CUDA graph only while no eager graph of the same parameters is
+alive.
 """
 from functools import partial
 from math import prod
@@ -12,8 +14,9 @@ from typing import Optional
 
 import torch
 import torch.nn as nn
-from torch.autograd import Function
+from torch.autograd import Function, forward_ad
 from torch.autograd.function import once_differentiable
+from torch.utils._device import DeviceContext
 
 from . import _abi, kernels
 
@@ -88,11 +91,20 @@ def embedding(tokens: torch.Tensor, weight: torch.Tensor, padding_idx: Optional[
 # ---------------------------------------------------------------------------------------------------
 
 
+def _watched():
+    """Whether something has to see torch's own operations: a compiler, a trace, a functional transform, forward-mode
+    derivatives, a dispatch or function mode (fake tensors, counters; a default device changes no operation here)."""
+    return (torch.compiler.is_compiling() or torch.jit.is_tracing() or torch._C._are_functorch_transforms_active()
+            or forward_ad._current_level >= 0 or torch._C._len_torch_dispatch_stack() > 0
+            or any(not isinstance(torch._C._get_function_stack_at(i), DeviceContext) for i in range(torch._C._len_torch_function_stack())))
+
+
 def _plain_cuda(x, *params):
-    """The kernels take CUDA tensors of one supported type, outside autocast (which would change the types) and outside
-    torch's functional transforms."""
-    return (x.is_cuda and all(p is None or (p.is_cuda and p.dtype in _DTYPES and p.device == x.device) for p in params)
-            and not torch.is_autocast_enabled('cuda') and not torch._C._are_functorch_transforms_active())
+    """The kernels take CUDA tensors of one supported type, no subclasses of torch's, outside autocast (which would change
+    the types) and where nothing watches torch's operations."""
+    return (not _watched() and x.is_cuda and type(x) in (torch.Tensor, nn.Parameter)
+            and all(p is None or (p.is_cuda and type(p) in (torch.Tensor, nn.Parameter) and p.dtype in _DTYPES and p.device == x.device)
+                    for p in params) and not torch.is_autocast_enabled('cuda'))
 
 
 # torch's own, as they were when this module was imported: a class that has been given another one keeps that
@@ -100,15 +112,18 @@ _TORCH_FORWARD = {kind: kind.forward for kind in (nn.LayerNorm, nn.Embedding)}
 
 
 def _layer_norm_layer(layer: nn.LayerNorm, x):
-    if type(layer).forward is _TORCH_FORWARD[nn.LayerNorm] and x.dtype in _DTYPES and 0 < prod(layer.normalized_shape) <= _abi.NORM_MAX_COLS and all(p is None or p.dtype == x.dtype for p in (layer.weight, layer.bias)) and _plain_cuda(
-            x, layer.weight, layer.bias):
-        return layer_norm(x, layer.normalized_shape, layer.weight, layer.bias, layer.eps)
+    shape, weight, bias = layer.normalized_shape, layer.weight, layer.bias
+    if (type(layer).forward is _TORCH_FORWARD[nn.LayerNorm] and _plain_cuda(x, weight, bias) and x.dtype in _DTYPES
+            and all(p is None or p.dtype == x.dtype for p in (weight, bias)) and 0 < prod(shape) <= _abi.NORM_MAX_COLS
+            and x.shape[-len(shape):] == shape):
+        return layer_norm(x, shape, weight, bias, layer.eps)
     return type(layer).forward(layer, x)
 
 
 def _embedding_layer(layer: nn.Embedding, tokens):
-    if (type(layer).forward is _TORCH_FORWARD[nn.Embedding] and tokens.dtype in (torch.int32, torch.int64) and layer.max_norm is None and not layer.sparse
-            and not layer.scale_grad_by_freq and layer.weight.numel() > 0 and _plain_cuda(tokens, layer.weight)):
+    if (type(layer).forward is _TORCH_FORWARD[nn.Embedding] and _plain_cuda(tokens, layer.weight)
+            and tokens.dtype in (torch.int32, torch.int64) and layer.max_norm is None and not layer.sparse
+            and not layer.scale_grad_by_freq and layer.weight.numel() > 0):
         return embedding(tokens, layer.weight, layer.padding_idx)
     return type(layer).forward(layer, tokens)
 
@@ -116,8 +131,11 @@ def _embedding_layer(layer: nn.Embedding, tokens):
 def use_kernels(module: nn.Module) -> int:
     """Run every ``nn.LayerNorm`` and ``nn.Embedding`` of ``module`` (subclasses that keep their ``forward`` included)
     through this package's kernels wherever those apply: CUDA tensors, one type for input and parameters, no autocast;
-    embeddings without ``max_norm``, ``sparse`` and ``scale_grad_by_freq``.  Other calls stay with torch.  A layer with a
-    ``forward`` of its own, set on the layer or on its class, keeps that.  Returns the number of layers."""
+    embeddings without ``max_norm``, ``sparse`` and ``scale_grad_by_freq``.  Other calls stay with torch: tensor subclasses,
+    forward-mode derivatives and functional transforms, compilation and tracing, calls under a dispatch or function mode.  A
+    layer with a ``forward`` of its own, set on the layer or on its class, keeps that.  (``torch.jit.script``
+    takes a module before this, not after; a shallow copy of a layer needs a call of its own.)  Returns the number of
+    layers."""
     count = 0
     for layer in module.modules():
         for kind, forward in ((nn.LayerNorm, _layer_norm_layer), (nn.Embedding, _embedding_layer)):

@@ -143,3 +143,21 @@ def test_a_class_keeps_a_forward_that_it_was_given(monkeypatch, kind, shape):
     assert F.use_kernels(late) == 0 and 'forward' not in late.__dict__
     monkeypatch.setattr(F, '_plain_cuda', lambda *a: True)    # as with CUDA tensors: the patch comes first all the same
     assert torch.equal(early(t), want)
+
+
+def test_layers_leave_fake_tensors_and_subclasses_to_torch(monkeypatch):
+    """A fake CUDA tensor has no memory that a kernel could take."""
+    from torch._subclasses.fake_tensor import FakeTensorMode
+    from elixir_b200 import functional as F, kernels as K
+
+    def never(*args, **kw):
+        raise AssertionError('a kernel was called')
+
+    for name in ('layer_norm_forward', 'embedding_forward'):
+        monkeypatch.setattr(K, name, never)
+    with FakeTensorMode():
+        model = nn.Sequential(nn.Embedding(10, 8, device='cuda'), nn.LayerNorm(8, device='cuda'))
+        assert F.use_kernels(model) == 2
+        out = model(torch.zeros(3, 4, dtype=torch.int64, device='cuda'))
+    assert out.shape == (3, 4, 8) and out.is_cuda
+    assert model[1](out).is_cuda    # outside the mode as well
