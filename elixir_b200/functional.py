@@ -4,7 +4,7 @@
 them (``use_kernels``), where the reference swaps in a fused layer norm (``elixir/kernels/layernorm.py:4``,
 ``elixir/hook/parameter.py:69-70``).  Statistics and sums are fp32, every output is rounded once, and both parameter
 gradients are summed in an order that the inputs alone fix.  CUDA tensors only.  ``layer_norm`` and ``embedding`` have first
-derivatives in reverse mode only; forward-mode derivatives of a module's layers stay with torch (``use_kernels``).  As with
+derivatives in reverse mode only; for anything else the layers of a module stay with torch (``use_kernels``).  As with
 every autograd function, a backward pass is captured into a CUDA graph only while no eager graph of the same parameters is
 alive.
 """
@@ -43,9 +43,30 @@ class _LayerNorm(Function):
                 None if dbias is None else dbias.view(ctx.bias_shape), None)
 
 
+class _LayerNormOfLayer(_LayerNorm):
+    """A backward pass that is going to be differentiated itself (``create_graph``) is torch's."""
+
+    @staticmethod
+    def backward(ctx, dy):
+        if not torch.is_grad_enabled():
+            return _LayerNorm.backward(ctx, dy)
+        x, weight, mean, rstd = ctx.saved_tensors
+        need_x, need_weight, need_bias = (need and t is not None for need, t in zip(ctx.needs_input_grad, (x, weight, ctx.bias_shape)))
+        rows = x.shape[:-1] + (1, )
+        dx, dweight, _ = torch.ops.aten.native_layer_norm_backward(dy, x, x.shape[-1:], mean.view(rows), rstd.view(rows),
+                                                                   None if weight is None else weight.flatten(), None,
+                                                                   [need_x, need_weight, False])
+        return (dx if need_x else None, dweight.view(weight.shape) if need_weight else None,
+                dy.reshape(-1, dy.shape[-1]).sum(0).view(ctx.bias_shape) if need_bias else None, None)
+
+
 def layer_norm(x: torch.Tensor, normalized_shape, weight: Optional[torch.Tensor] = None,
                bias: Optional[torch.Tensor] = None, eps: float = 1e-5) -> torch.Tensor:
     """``torch.nn.functional.layer_norm`` on this package's kernels.  ``weight`` and ``bias`` have the type of ``x``."""
+    return _apply_layer_norm(_LayerNorm, x, normalized_shape, weight, bias, eps)
+
+
+def _apply_layer_norm(function, x, normalized_shape, weight, bias, eps):
     shape = (normalized_shape, ) if isinstance(normalized_shape, int) else tuple(normalized_shape)
     if not shape or x.shape[-len(shape):] != shape or x.dim() < len(shape):
         raise ValueError(f'normalized_shape {shape} does not end the shape {tuple(x.shape)}')
@@ -57,7 +78,7 @@ def layer_norm(x: torch.Tensor, normalized_shape, weight: Optional[torch.Tensor]
         flat = flat.flatten(-len(shape))
     # the parameters themselves, not views of them: the memory of a chunk may be another by the time of the backward pass
     weight, bias = (t if t is None else t.contiguous() for t in (weight, bias))
-    return _LayerNorm.apply(flat, weight, bias, eps).view(x.shape)
+    return function.apply(flat, weight, bias, eps).view(x.shape)
 
 
 class _Embedding(Function):
@@ -75,15 +96,34 @@ class _Embedding(Function):
         return None, kernels.embedding_backward(tokens, dout.contiguous(), ctx.vocab, ctx.scale, ctx.padding_idx), None, None
 
 
+class _EmbeddingOfLayer(_Embedding):
+    """As ``_LayerNormOfLayer``: torch's, for a scale of 1."""
+
+    @staticmethod
+    def backward(ctx, dout):
+        if not torch.is_grad_enabled():
+            return _Embedding.backward(ctx, dout)
+        tokens, = ctx.saved_tensors
+        keep = (tokens >= 0) & (tokens < ctx.vocab)    # torch's operator takes tokens of the table only
+        if ctx.padding_idx is not None:
+            keep &= tokens != ctx.padding_idx
+        dout = torch.where(keep.unsqueeze(-1), dout, torch.zeros_like(dout))
+        return None, torch.ops.aten.embedding_dense_backward(dout, torch.where(keep, tokens, 0), ctx.vocab, -1, False), None, None
+
+
 def embedding(tokens: torch.Tensor, weight: torch.Tensor, padding_idx: Optional[int] = None, scale: float = 1.0) -> torch.Tensor:
     """``scale * weight[tokens]``.  As with ``torch.nn.functional.embedding``, ``padding_idx`` (negative values count from
     the end) names the token whose row gets no gradient; the gradient is dense.  A token outside the table, which torch
     answers with a device assertion, reads as a row of NaN here: the overflow probe then skips the step."""
+    return _apply_embedding(_Embedding, tokens, weight, padding_idx, scale)
+
+
+def _apply_embedding(function, tokens, weight, padding_idx, scale=1.0):
     if padding_idx is not None:
         if not -weight.shape[0] <= padding_idx < weight.shape[0]:
             raise ValueError('padding_idx outside the table')
         padding_idx %= weight.shape[0]
-    return _Embedding.apply(tokens.contiguous(), weight.contiguous(), padding_idx, float(scale))
+    return function.apply(tokens.contiguous(), weight.contiguous(), padding_idx, float(scale))
 
 
 # ---------------------------------------------------------------------------------------------------
@@ -116,7 +156,7 @@ def _layer_norm_layer(layer: nn.LayerNorm, x):
     if (type(layer).forward is _TORCH_FORWARD[nn.LayerNorm] and _plain_cuda(x, weight, bias) and x.dtype in _DTYPES
             and all(p is None or p.dtype == x.dtype for p in (weight, bias)) and 0 < prod(shape) <= _abi.NORM_MAX_COLS
             and x.shape[-len(shape):] == shape):
-        return layer_norm(x, shape, weight, bias, layer.eps)
+        return _apply_layer_norm(_LayerNormOfLayer, x, shape, weight, bias, layer.eps)
     return type(layer).forward(layer, x)
 
 
@@ -124,7 +164,7 @@ def _embedding_layer(layer: nn.Embedding, tokens):
     if (type(layer).forward is _TORCH_FORWARD[nn.Embedding] and _plain_cuda(tokens, layer.weight)
             and tokens.dtype in (torch.int32, torch.int64) and layer.max_norm is None and not layer.sparse
             and not layer.scale_grad_by_freq and layer.weight.numel() > 0):
-        return embedding(tokens, layer.weight, layer.padding_idx)
+        return _apply_embedding(_EmbeddingOfLayer, tokens, layer.weight, layer.padding_idx)
     return type(layer).forward(layer, tokens)
 
 
@@ -132,10 +172,10 @@ def use_kernels(module: nn.Module) -> int:
     """Run every ``nn.LayerNorm`` and ``nn.Embedding`` of ``module`` (subclasses that keep their ``forward`` included)
     through this package's kernels wherever those apply: CUDA tensors, one type for input and parameters, no autocast;
     embeddings without ``max_norm``, ``sparse`` and ``scale_grad_by_freq``.  Other calls stay with torch: tensor subclasses,
-    forward-mode derivatives and functional transforms, compilation and tracing, calls under a dispatch or function mode.  A
-    layer with a ``forward`` of its own, set on the layer or on its class, keeps that.  (``torch.jit.script``
-    takes a module before this, not after; a shallow copy of a layer needs a call of its own.)  Returns the number of
-    layers."""
+    forward-mode derivatives and functional transforms, compilation and tracing, calls under a dispatch or function mode; so
+    do the operations of a backward pass with ``create_graph``.  A layer with a ``forward`` of its own, set on the layer or
+    on its class, keeps that.  (``torch.jit.script`` takes a module before this, not after; a shallow copy of a layer needs a
+    call of its own.)  Returns the number of layers."""
     count = 0
     for layer in module.modules():
         for kind, forward in ((nn.LayerNorm, _layer_norm_layer), (nn.Embedding, _embedding_layer)):

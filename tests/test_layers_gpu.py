@@ -99,3 +99,37 @@ def test_fake_tensors_dispatch_modes_and_compilation(models, launches):
     # (the check of a trace calls the module itself once more)
     assert torch.equal(torch.jit.trace(ours, (tokens, ), check_trace=False)(tokens), want)
     assert not launches
+
+
+def test_second_derivatives(models, launches):
+    """A penalty on the gradients, its own gradients with respect to every parameter: within the roundings of an fp32
+    evaluation of torch's, whose order of sums differs in the first forward pass only."""
+    theirs, ours, tokens = models
+    weight = torch.randn(3, 7, 40, device=tokens.device)
+    grads = []
+    for model in (theirs, ours, copy.deepcopy(theirs).double()):
+        dtype = model.norm.weight.dtype
+        loss = torch.tanh(model(tokens) * weight.to(dtype)).sum()
+        first = torch.autograd.grad(loss, list(model.parameters()), create_graph=True)
+        second = torch.autograd.grad(sum(g.pow(2).sum() for g in first), list(model.parameters()))
+        grads.append((first, second))
+    assert len(launches) == 4
+    for torchs, mine, exact in zip(*(first + second for first, second in grads)):
+        # a few hundred roundings of numbers of the gradients' size lie between the tokens and a second derivative
+        assert mine.shape == exact.shape and bool((mine.double() - exact).norm() <= 1000 * 2.0**-24 * exact.norm())
+    assert bool((grads[1][0][0][2] == 0).all()) and bool((grads[1][1][0][2] == 0).all())    # the padding token
+
+
+def test_second_derivatives_past_a_token_outside_the_table(cuda):
+    """Such a token reads as a row of NaN and adds to no row, in a differentiated backward pass as in a plain one."""
+    from elixir_b200 import functional as F
+    layer = nn.Embedding(10, 8).to(cuda)
+    F.use_kernels(layer)
+    scale = torch.ones(4, 8, device=cuda, requires_grad=True)
+    out = layer(torch.tensor([1, 10, -1, 3], device=cuda)).nan_to_num(0.0)
+    g, = torch.autograd.grad((out * scale).sum(), layer.weight, create_graph=True)
+    want = torch.zeros(10, 8, device=cuda)
+    want[[1, 3]] = 1
+    assert torch.equal(g, want)
+    twice, = torch.autograd.grad(g.sum(), scale)
+    assert torch.equal(twice, torch.tensor([1.0, 0, 0, 1], device=cuda)[:, None].expand(4, 8))
