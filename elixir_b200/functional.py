@@ -51,7 +51,8 @@ class _LayerNormOfLayer(_LayerNorm):
         if not torch.is_grad_enabled():
             return _LayerNorm.backward(ctx, dy)
         x, weight, mean, rstd = ctx.saved_tensors
-        need_x, need_weight, need_bias = (need and t is not None for need, t in zip(ctx.needs_input_grad, (x, weight, ctx.bias_shape)))
+        need_x, need_weight = ctx.needs_input_grad[0], ctx.needs_input_grad[1] and weight is not None
+        need_bias = ctx.needs_input_grad[2] and ctx.bias_shape is not None
         rows = x.shape[:-1] + (1, )
         dx, dweight, _ = torch.ops.aten.native_layer_norm_backward(dy, x, x.shape[-1:], mean.view(rows), rstd.view(rows),
                                                                    None if weight is None else weight.flatten(), None,
@@ -136,15 +137,16 @@ def _watched():
     derivatives, a dispatch or function mode (fake tensors, counters; a default device changes no operation here)."""
     return (torch.compiler.is_compiling() or torch.jit.is_tracing() or torch._C._are_functorch_transforms_active()
             or forward_ad._current_level >= 0 or torch._C._len_torch_dispatch_stack() > 0
-            or any(not isinstance(torch._C._get_function_stack_at(i), DeviceContext) for i in range(torch._C._len_torch_function_stack())))
+            or any(not isinstance(torch._C._get_function_stack_at(i), DeviceContext)
+                   for i in range(torch._C._len_torch_function_stack())))
 
 
 def _plain_cuda(x, *params):
     """The kernels take CUDA tensors of one supported type, no subclasses of torch's, outside autocast (which would change
     the types) and where nothing watches torch's operations."""
     return (not _watched() and x.is_cuda and type(x) in (torch.Tensor, nn.Parameter)
-            and all(p is None or (p.is_cuda and type(p) in (torch.Tensor, nn.Parameter) and p.dtype in _DTYPES and p.device == x.device)
-                    for p in params) and not torch.is_autocast_enabled('cuda'))
+            and all(p is None or (p.is_cuda and type(p) in (torch.Tensor, nn.Parameter) and p.dtype in _DTYPES
+                                  and p.device == x.device) for p in params) and not torch.is_autocast_enabled('cuda'))
 
 
 # torch's own, as they were when this module was imported: a class that has been given another one keeps that

@@ -120,6 +120,26 @@ def test_second_derivatives(models, launches):
     assert bool((grads[1][0][0][2] == 0).all()) and bool((grads[1][1][0][2] == 0).all())    # the padding token
 
 
+@pytest.mark.parametrize('dtype', [torch.float16, torch.bfloat16])
+def test_second_derivatives_in_16_bits(models, dtype):
+    """Those of the same layers in torch, from the same values.  After the forward pass, whose results differ by a rounding
+    here and there, both run the same operators."""
+    theirs, ours, tokens = models
+    theirs, ours = theirs.to(dtype), ours.to(dtype)
+    grads = []
+    for model in (theirs, ours):
+        first = torch.autograd.grad(torch.tanh(model(tokens)).float().sum(), list(model.parameters()), create_graph=True)
+        grads.append(first + torch.autograd.grad(sum(g.float().pow(2).sum() for g in first), list(model.parameters())))
+    for torchs, mine in zip(*grads):
+        # torch's operators leave fp16's range on the way to some second derivatives, for its own layers as well
+        assert mine.dtype == dtype and torch.equal(torch.isfinite(mine), torch.isfinite(torchs))
+        mine, torchs = (torch.where(torch.isfinite(t), t, 0.0).double() for t in (mine, torchs))
+        # some thirty roundings of half a step, on both sides
+        assert bool((mine - torchs).norm() <= 60 * torch.finfo(dtype).eps / 2 * torchs.norm())
+    if dtype == torch.bfloat16:
+        assert all(bool(torch.isfinite(g).all()) for g in grads[1])
+
+
 def test_second_derivatives_past_a_token_outside_the_table(cuda):
     """Such a token reads as a row of NaN and adds to no row, in a differentiated backward pass as in a plain one."""
     from elixir_b200 import functional as F
