@@ -79,6 +79,37 @@ def test_a_vocabulary_of_three_digits(cuda):
     _case(cuda, 2500, 17_000_001, 8, spread='even', seed=5)
 
 
+@pytest.mark.parametrize('n', [65536, 65537, 131072, 200001])    # a cluster sorts 65536 at most
+@pytest.mark.parametrize('spread', ['zipf', 'few', 'even'])
+@pytest.mark.parametrize('vocab', [1000, 50257, 70001])    # two and three digits
+def test_more_tokens_than_a_cluster_sorts(cuda, n, spread, vocab):
+    """Padding and tokens outside the table among them.  The sort is stable: tokens that come sorted already, with their rows,
+    give the same bits."""
+    from elixir_b200 import kernels as K
+    tokens = _tokens(n, vocab, spread, torch.int64, n)
+    gen = torch.Generator().manual_seed(n)
+    tokens[torch.randint(n, (50, ), generator=gen)] = vocab + 3
+    tokens[torch.randint(n, (50, ), generator=gen)] = -1
+    padding = int(tokens[tokens >= 0][0])
+    tokens = tokens.to(cuda)
+    dout = torch.randn(n, 24, device=cuda, generator=torch.Generator(device=cuda).manual_seed(n)).half()
+    got = K.embedding_backward(tokens, dout, vocab, 1.0, padding)
+    _check_grad(got, tokens, dout, vocab, 1.0, padding)
+    assert bool((got[padding] == 0).all())
+    key = torch.where((tokens < 0) | (tokens >= vocab) | (tokens == padding), vocab, tokens)
+    order = torch.sort(key, stable=True).indices
+    assert torch.equal(K.embedding_backward(tokens[order], dout[order], vocab, 1.0, padding), got)
+    assert torch.equal(K.embedding_backward(tokens.int(), dout, vocab, 1.0, padding), got)
+
+
+@pytest.mark.parametrize('n', [65537, 70000])
+def test_more_tokens_than_a_cluster_sorts_by_four_digits(cuda, n):
+    from elixir_b200 import kernels as K
+    tokens, dout, got = _case(cuda, n, 2**24 + 51, 4, spread='even', seed=6)
+    order = torch.sort(tokens, stable=True).indices
+    assert torch.equal(K.embedding_backward(tokens[order], dout[order], 2**24 + 51), got)
+
+
 @pytest.mark.parametrize('dtype', [torch.float16, torch.bfloat16, torch.float32])
 @pytest.mark.parametrize('width', [1, 2, 3, 4, 7, 8, 12, 64, 100, 257, 1600, 2049, 5120])
 def test_widths(cuda, dtype, width):
