@@ -104,6 +104,61 @@ def test_rows(cuda, dtype, rows, cols):
     _run(*_inputs(rows, cols, dtype, 'both', seed=rows))
 
 
+@pytest.mark.parametrize('dtype', [torch.float16, torch.bfloat16, torch.float32])
+@pytest.mark.parametrize('cols', [5120, 8193, 9216, 9217, 12288, 16384, 16392, 20001])
+def test_many_wide_rows(cuda, dtype, cols):
+    """Several rows per block where a row takes the whole block: every block comes round four or five times."""
+    _run(*_inputs(601, cols, dtype, 'both', seed=cols))
+
+
+@pytest.mark.parametrize('dtype', [torch.float16, torch.float32])
+@pytest.mark.parametrize('rows', [149, 593, 4001])
+def test_many_narrow_rows_and_rows_off_alignment(cuda, dtype, rows):
+    """Several groups per block in the kernels that access one element at a time."""
+    for cols in (1, 3, 17, 31):
+        _run(*_inputs(rows, cols, dtype, 'both', seed=cols))
+    for cols in (65, 1601):
+        _run(*_inputs(rows, cols, dtype, 'both', seed=cols, offset=1))
+
+
+@pytest.mark.parametrize('dtype', [torch.float16, torch.bfloat16, torch.float32])
+@pytest.mark.parametrize('offset', [1, 3, 7])
+@pytest.mark.parametrize('rows,cols', [(1, 33), (5, 65), (601, 1111), (37, 1600), (149, 8201), (7, 16000)])
+def test_all_arrays_at_one_distance_from_a_boundary(cuda, dtype, offset, rows, cols):
+    """Through the C entry points, which take such arrays: x, y, dy and dx begin at the same odd place, the parameters at
+    others.  What lies around the arrays is left as it was."""
+    from elixir_b200 import _lib, kernels as K
+    lib, n, mark, room = _lib.get(), rows * cols, 123.0, 16
+
+    def at(t):
+        buffer = torch.full((room + offset + t.numel() + room, ), mark, dtype=t.dtype, device=cuda)
+        inside = buffer[room + offset:room + offset + t.numel()]
+        inside.copy_(t.reshape(-1))
+        return buffer, inside
+
+    x, w, b, dy = _inputs(rows, cols, dtype, 'both', seed=cols)
+    empty = torch.zeros(n, dtype=dtype, device=cuda)
+    rooms = {k: at(t) for k, t in dict(x=x, dy=dy, y=empty, dx=empty, dw=w, db=b).items()}
+    p = {k: inside.data_ptr() for k, (_, inside) in rooms.items()}
+    mean, rstd = torch.empty(rows, device=cuda), torch.empty(rows, device=cuda)
+    code, stream = K.dtype_code(dtype), torch.cuda.current_stream(cuda).cuda_stream
+    assert lib.elx_layer_norm_forward(p['x'], w.data_ptr(), b.data_ptr(), code, rows, cols, 1e-5, p['y'], mean.data_ptr(),
+                                      rstd.data_ptr(), stream) == 0
+    size = lib.elx_layer_norm_backward_workspace(rows, cols)
+    space = torch.full((size + 64, ), 77, dtype=torch.uint8, device=cuda)
+    assert lib.elx_layer_norm_backward(p['dy'], p['x'], w.data_ptr(), mean.data_ptr(), rstd.data_ptr(), code, rows, cols, p['dx'],
+                                       p['dw'], p['db'], space.data_ptr(), size, stream) == 0
+    want = _reference(x, w, b, dy, 1e-5, rows_chain=rows / 64 + 100)
+    _check(mean, *want['mean'], torch.float32)
+    _check(rstd, *want['rstd'], torch.float32)
+    for key in ('y', 'dx', 'dw', 'db'):
+        _check(rooms[key][1].view(want[key][0].shape), *want[key], dtype)
+    assert torch.equal(rooms['x'][1], x.view(-1)) and torch.equal(rooms['dy'][1], dy.view(-1))
+    for buffer, inside in rooms.values():
+        assert bool((buffer[:room + offset] == mark).all()) and bool((buffer[room + offset + inside.numel():] == mark).all())
+    assert bool((space[size:] == 77).all())
+
+
 @pytest.mark.parametrize('affine', ['none', 'weight', 'both'])
 @pytest.mark.parametrize('offset', [0, 1, 2, 4])
 @pytest.mark.parametrize('dtype', [torch.float16, torch.float32])
