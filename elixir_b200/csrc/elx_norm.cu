@@ -694,49 +694,26 @@ __global__ void __launch_bounds__(1024) norm_columns_kernel(const float* __restr
 
 int round32(int n) { return (n + 31) / 32 * 32; }
 
-template <int DT, int VEC, int VPL>
+template <int DT, int VEC, int VPL, bool ONE>
 int launch_forward(const NormArgs& a, int warps, cudaStream_t s) {
-    if (warps == 1) {
-        const int64_t grid = (a.rows + 3) / 4;
-        if (grid > 0x7FFFFFFF) return ELX_ERR_CAPACITY;
-        norm_forward_kernel<DT, VEC, VPL, true><<<static_cast<unsigned>(grid), 128, 0, s>>>(a);
-    } else {
-        if (a.rows > 0x7FFFFFFF || 32 * warps > max_threads(VEC, VPL)) return ELX_ERR_CAPACITY;
-        norm_forward_kernel<DT, VEC, VPL, false><<<static_cast<unsigned>(a.rows), 32 * warps, 0, s>>>(a);
-    }
+    const int64_t grid = ONE ? (a.rows + 3) / 4 : a.rows;
+    if (grid > 0x7FFFFFFF || (!ONE && 32 * warps > max_threads(VEC, VPL))) return ELX_ERR_CAPACITY;
+    norm_forward_kernel<DT, VEC, VPL, ONE><<<static_cast<unsigned>(grid), ONE ? 128 : 32 * warps, 0, s>>>(a);
     return record_cuda(cudaGetLastError());
 }
 
-// Pieces per lane are rounded up to one of these.
-template <int VEC>
-int round_pieces(int each) {
-    constexpr int wide[] = {1, 2, 3, 4, 5, 6, 7, 8, 10, 12, 16, 20}, single[] = {1, 2, 4, 8, 16, 24, 32, 40};
-    if constexpr (VEC == 1) {
-        for (const int v : single)
-            if (each <= v) return v;
-    } else {
-        for (const int v : wide)
-            if (each <= v) return v;
-    }
-    return 0;
-}
-
 // Warps per row, by its width alone, so that a row's result does not depend on how many rows the call has: one, where the
-// row fits a warp's registers in few pieces per lane, else as many as give each lane four.  Measured (GB/s of x and y, fp16):
-// 8192 x 1600 in one warp 3740, in two 3460; 16384 x 4096 in one 3090, two 4070, four 5160, eight 3740.  0: no such kernel.
+// row fits a warp's registers in few pieces per lane, else as many as give each lane four (16, of one element), else 16 warps
+// of as many as their registers hold.  Measured (GB/s of x and y, fp16): 8192 x 1600 in one warp 3740, in two 3460;
+// 16384 x 4096 in one 3090, two 4070, four 5160, eight 3740.  On both sides of seven pieces, fp16: 32768 x 1792 (seven) 49 us
+// in one warp, 53 us in two; 8192 x 1800 (eight) 22.3 us in one, 20.6 us in two, though 32768 rows of it take 52.5 and 53.6 us.
+// 0: no such kernel.
 template <int VEC>
-int forward_warps(int pieces, int* each) {
-    constexpr int kAlone = VEC == 1 ? 40 : 7, kEach = VEC == 1 ? 16 : 4;
-    int warps = pieces <= 32 * kAlone ? 1 : (pieces + 32 * kEach - 1) / (32 * kEach);
-    if (warps > 32) warps = 16;
-    for (; warps >= 1; warps /= 2) {
-        const int e = round_pieces<VEC>((pieces + 32 * warps - 1) / (32 * warps));
-        if (e == 0) return 0;
-        if (warps > 1 && 32 * warps > max_threads(VEC, e)) continue;
-        *each = e;
-        return warps;
-    }
-    return 0;
+int forward_warps(int pieces) {
+    constexpr int kAlone = VEC == 1 ? 40 : 7, kEach = VEC == 1 ? 16 : 4, kMost = VEC == 1 ? 40 : 10;
+    if (pieces <= 32 * kAlone) return 1;
+    const int warps = (pieces + 32 * kEach - 1) / (32 * kEach);
+    return warps <= 32 ? warps : pieces <= 32 * 16 * kMost ? 16 : 0;
 }
 
 // Blocks of a kernel whose groups of threads walk over rows: one per SM of a B200 at most, whatever the device, so that the
@@ -763,40 +740,40 @@ int launch_forward_odd(NormArgs a, cudaStream_t s) {
 template <int DT>
 int forward_dt(const NormArgs& a, bool wide_ok, bool same_mis, cudaStream_t s) {
     constexpr int V = Wide<DT>::kVec;
-    int each = 0;
     if (!wide_ok && same_mis && a.cols >= 4 * V) {
         const int pieces = (a.cols + 2 * V - 2) / V;
         if (pieces <= 32) return launch_forward_odd<DT, 1>(a, s);
         if (pieces <= 512) return launch_forward_odd<DT, 2>(a, s);
         if (pieces <= 2048) return launch_forward_odd<DT, 4>(a, s);
     }
-    const int warps = wide_ok ? forward_warps<V>(a.cols / V, &each) : forward_warps<1>(a.cols, &each);
-    if (warps && wide_ok) {
+    const int warps = wide_ok ? forward_warps<V>(a.cols / V) : forward_warps<1>(a.cols);
+    const int each = warps ? ((wide_ok ? a.cols / V : a.cols) + 32 * warps - 1) / (32 * warps) : 0;   // pieces per lane
+    if (wide_ok && warps == 1) {
         switch (each) {
-            case 1: return launch_forward<DT, V, 1>(a, warps, s);
-            case 2: return launch_forward<DT, V, 2>(a, warps, s);
-            case 3: return launch_forward<DT, V, 3>(a, warps, s);
-            case 4: return launch_forward<DT, V, 4>(a, warps, s);
-            case 5: return launch_forward<DT, V, 5>(a, warps, s);
-            case 6: return launch_forward<DT, V, 6>(a, warps, s);
-            case 7: return launch_forward<DT, V, 7>(a, warps, s);
-            case 8: return launch_forward<DT, V, 8>(a, warps, s);
-            case 10: return launch_forward<DT, V, 10>(a, warps, s);
-            case 12: return launch_forward<DT, V, 12>(a, warps, s);
-            case 16: return launch_forward<DT, V, 16>(a, warps, s);
-            case 20: return launch_forward<DT, V, 20>(a, warps, s);
+            case 1: return launch_forward<DT, V, 1, true>(a, warps, s);
+            case 2: return launch_forward<DT, V, 2, true>(a, warps, s);
+            case 3: return launch_forward<DT, V, 3, true>(a, warps, s);
+            case 4: return launch_forward<DT, V, 4, true>(a, warps, s);
+            case 5: return launch_forward<DT, V, 5, true>(a, warps, s);
+            case 6: return launch_forward<DT, V, 6, true>(a, warps, s);
+            case 7: return launch_forward<DT, V, 7, true>(a, warps, s);
         }
+    } else if (wide_ok && warps) {
+        if (each <= 3) return launch_forward<DT, V, 3, false>(a, warps, s);
+        if (each == 4) return launch_forward<DT, V, 4, false>(a, warps, s);
+        return launch_forward<DT, V, 10, false>(a, warps, s);
+    } else if (warps == 1) {
+        if (each == 1) return launch_forward<DT, 1, 1, true>(a, warps, s);
+        if (each == 2) return launch_forward<DT, 1, 2, true>(a, warps, s);
+        if (each <= 4) return launch_forward<DT, 1, 4, true>(a, warps, s);
+        if (each <= 8) return launch_forward<DT, 1, 8, true>(a, warps, s);
+        if (each <= 16) return launch_forward<DT, 1, 16, true>(a, warps, s);
+        if (each <= 24) return launch_forward<DT, 1, 24, true>(a, warps, s);
+        if (each <= 32) return launch_forward<DT, 1, 32, true>(a, warps, s);
+        return launch_forward<DT, 1, 40, true>(a, warps, s);
     } else if (warps) {
-        switch (each) {
-            case 1: return launch_forward<DT, 1, 1>(a, warps, s);
-            case 2: return launch_forward<DT, 1, 2>(a, warps, s);
-            case 4: return launch_forward<DT, 1, 4>(a, warps, s);
-            case 8: return launch_forward<DT, 1, 8>(a, warps, s);
-            case 16: return launch_forward<DT, 1, 16>(a, warps, s);
-            case 24: return launch_forward<DT, 1, 24>(a, warps, s);
-            case 32: return launch_forward<DT, 1, 32>(a, warps, s);
-            case 40: return launch_forward<DT, 1, 40>(a, warps, s);
-        }
+        if (each <= 16) return launch_forward<DT, 1, 16, false>(a, warps, s);
+        return launch_forward<DT, 1, 40, false>(a, warps, s);
     }
     if (a.rows > 0x7FFFFFFF) return ELX_ERR_CAPACITY;
     norm_forward_wide_kernel<DT><<<static_cast<unsigned>(a.rows), 1024, 0, s>>>(a);

@@ -105,6 +105,21 @@ def test_rows(cuda, dtype, rows, cols):
 
 
 @pytest.mark.parametrize('dtype', [torch.float16, torch.bfloat16, torch.float32])
+@pytest.mark.parametrize('lanes,pieces', [(32, p) for p in (1, 2, 3, 4, 5, 6, 7)] + [(64, 4), (96, 3), (1024, 4), (512, 10)])
+def test_every_forward_kernel_of_16_byte_pieces(cuda, dtype, lanes, pieces):
+    """The widest row of each number of lanes and pieces per lane, and the first row past it."""
+    for cols in (lanes * pieces * 16 // dtype.itemsize, (lanes * pieces + 1) * 16 // dtype.itemsize):
+        _run(*_inputs(9, cols, dtype, 'both', seed=cols))
+
+
+@pytest.mark.parametrize('dtype', [torch.float16, torch.bfloat16, torch.float32])
+@pytest.mark.parametrize('cols', [32, 64, 128, 256, 512, 768, 1024, 1280, 16384, 20480])
+def test_every_forward_kernel_of_single_elements(cuda, dtype, cols):
+    for past in (0, 1):
+        _run(*_inputs(9, cols + past, dtype, 'both', seed=cols, offset=1))
+
+
+@pytest.mark.parametrize('dtype', [torch.float16, torch.bfloat16, torch.float32])
 @pytest.mark.parametrize('cols', [5120, 8193, 9216, 9217, 12288, 16384, 16392, 20001])
 def test_many_wide_rows(cuda, dtype, cols):
     """Several rows per block where a row takes the whole block: every block comes round four or five times."""
