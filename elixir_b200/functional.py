@@ -135,10 +135,11 @@ def _apply_embedding(function, tokens, weight, padding_idx, scale=1.0):
 def _watched():
     """Whether something has to see torch's own operations: a compiler, a trace, a functional transform, forward-mode
     derivatives, a dispatch or function mode (fake tensors, counters; a default device changes no operation here)."""
-    return (torch.compiler.is_compiling() or torch.jit.is_tracing() or torch._C._are_functorch_transforms_active()
+    return (torch.compiler.is_compiling() or torch._C._is_tracing() or torch._C._are_functorch_transforms_active()
             or forward_ad._current_level >= 0 or torch._C._len_torch_dispatch_stack() > 0
-            or any(not isinstance(torch._C._get_function_stack_at(i), DeviceContext)
-                   for i in range(torch._C._len_torch_function_stack())))
+            or (torch._C._len_torch_function_stack() > 0 and any(
+                not isinstance(torch._C._get_function_stack_at(i), DeviceContext)
+                for i in range(torch._C._len_torch_function_stack()))))
 
 
 def _plain_cuda(x, *params):
