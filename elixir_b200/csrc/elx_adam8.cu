@@ -708,7 +708,7 @@ __device__ __forceinline__ void pack_pair(const float* __restrict__ x, uint8_t* 
 }
 
 // Bound by the bytes: 8 in and 2 out per element; 64 Mi elements in 106 us (6.4 TB/s).  Back into fp32: 110 us (6.1 TB/s),
-// into bf16 70 us (5.8 TB/s).
+// into bf16 70 us (5.8 TB/s; that form spills 20 bytes per thread).
 __global__ void __launch_bounds__(kConvThreads) pack_kernel(const float* __restrict__ m, const float* __restrict__ v, int64_t n,
                                                             uint8_t* state_m, uint8_t* state_v, int vec) {
     const int64_t pairs = (n + kPair - 1) / kPair, stride = static_cast<int64_t>(gridDim.x) * (kConvThreads / 32);

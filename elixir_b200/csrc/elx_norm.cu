@@ -305,7 +305,9 @@ __device__ __forceinline__ float group_sum(float v, float* s, int id, int thread
 // Rows of a width that 16-byte pieces do not divide.  Groups of threads walk over rows that all begin at one distance from
 // a 16-byte boundary (their number is a multiple of V), so a thread's columns, weights and biases stay the same, and x and y
 // move in 16-byte pieces but for the two ends of a row.  8192 x 1111: fp16 24 us (31 us with an access per element), and
-// 8192 x 1601 fp32 37 us.  Bound by instructions: 31 per element, half of them for the ends of the rows.
+// 8192 x 1601 fp32 37 us.  Bound by instructions: 31 per element, half of them for the ends of the rows; and row, next row,
+// parameters and spans do not fit the registers: with two and four pieces per thread the 16-bit forms spill 180 to 212 bytes
+// and read 228 to 240 back.
 template <int DT, int VPL>
 __global__ void __launch_bounds__(512, VPL > 2 ? 1 : 2) norm_forward_odd_kernel(const NormArgs a) {
     constexpr int VEC = Wide<DT>::kVec;
@@ -428,7 +430,8 @@ __global__ void __launch_bounds__(1024) norm_forward_wide_kernel(const NormArgs 
 // as zero gradients.
 // With norm_columns_kernel, fp16: 8192 x 1600 23.5 us (3.3 TB/s), 16384 x 2048 41.8 us (4.8 TB/s), 16384 x 4096 78 us
 // (5.2 TB/s); bound by what a row waits for: its loads, one barrier, its sums.  Rows of more than 1024 pieces (NEXT off) lose
-// what is not on its way early: 4096 x 9216 113 us (2.0 TB/s).
+// what is not on its way early: 4096 x 9216 113 us (2.0 TB/s); the 16-bit forms of these spill as well, 104 to 296 bytes (132 to
+// 664 read back), and the odd ones of narrower rows up to 32.
 // VPL 1 up to 96 pieces: 32768 x 768 fp16 37 us against 39 with two per thread, 65536 x 256 28.6 us against 31.4 in 512 threads;
 // wider rows lose more by another warp's part of each row's sums (16384 x 1600 40 us with two per thread, 47 with one, 42 with
 // three).
@@ -635,6 +638,7 @@ __global__ void __launch_bounds__(backward_threads(VPL), 1) norm_backward_kernel
 }
 
 // Wide rows: dx row by row, and the column sums in a pass of their own, an access per element (1000 x 40000 fp16: 228 us).
+// fp32 rows come here from 8196 columns on: 4096 x 9216 215 us, where a pass over the bytes takes 70.
 template <int DT>
 __global__ void __launch_bounds__(1024) norm_backward_wide_kernel(const NormArgs a) {
     __shared__ float s_sum[2 * 32];

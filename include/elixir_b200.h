@@ -539,9 +539,9 @@ int64_t elx_moment_state_bytes(int64_t n);
  * working copies only.  An inf or a NaN costs its whole block: where a gradient is not finite, or a finite one's square
  * passes fp32's range (|g| above about 5.8e20 after unscaling, with beta2 = 0.999), the block's exponent becomes 255, all
  * 256 elements of that moment read as NaN and the next update makes their parameters NaN.  ELX_STAT_LATE_INF and late_inf
- * are raised by every update that leaves such a block.  Root and division of the parameter's step are approximate (within 1e-6 relative); "math_mode"
- * does not apply.  All pointers of a descriptor should be 32-byte aligned; other alignments are handled element by
- * element.
+ * are raised by every update that leaves such a block.  Root and division of the parameter's step are approximate (within
+ * 1e-6 relative); "math_mode" does not apply.  All pointers of a descriptor should be 32-byte aligned; other alignments are
+ * handled element by element.
  */
 int elx_adam8_multi(const ElxChunkDesc* descs, int first, int count, int64_t n_tiles, int dtype, const ElxSeg* segs,
                     const ElxHyper* hyper, int n_groups, ElxCtl* ctl, void* stream);
@@ -565,7 +565,9 @@ int elx_moments_unpack(const void* state_m, const void* state_v, int64_t n, int 
  * weight, bias: `cols` elements or NULL (1 and 0).  Arrays need the alignment of their element; 16-byte accesses are
  * used when every row starts on a 16-byte boundary.  rows = 0 is allowed; 1 <= cols <= ELX_NORM_MAX_COLS.
  * elx_layer_norm_backward: dx, and the sums over the rows dweight = sum dy xhat and dbias = sum dy (each `cols`
- * elements, NULL = not wanted), in an order that depends on rows and cols alone.  The sums need a workspace of
+ * elements, NULL = not wanted).  Every sum is taken in an order that the type, rows, cols and the arrays' alignment to 16
+ * bytes fix (they choose the kernel), so a call that is repeated gives the same bits; in rows that 16-byte pieces do not
+ * divide it also depends on the row's index, so two equal rows may differ in the last bit.  The sums need a workspace of
  * elx_layer_norm_backward_workspace(rows, cols) bytes, 16-byte aligned, not shared with a call that may run at the
  * same time; without them it may be NULL.  y and dx must not overlap the inputs.
  */
