@@ -150,8 +150,14 @@ def _plain_cuda(x, *params):
                                   and p.device == x.device) for p in params) and not torch.is_autocast_enabled('cuda'))
 
 
-# torch's own, as they were when this module was imported: a class that has been given another one keeps that
-_TORCH_FORWARD = {kind: kind.forward for kind in (nn.LayerNorm, nn.Embedding)}
+def _torch_forward(kind):
+    """The ``forward`` of a class of torch's, or None where a program has given it another one."""
+    home = getattr(kind.forward, '__globals__', {}).get('__name__')
+    return kind.forward if home == kind.__module__ else None
+
+
+# as they are when this module is imported: a class that has been given another one, before or after, keeps that
+_TORCH_FORWARD = {kind: _torch_forward(kind) for kind in (nn.LayerNorm, nn.Embedding)}
 
 
 def _layer_norm_layer(layer: nn.LayerNorm, x):

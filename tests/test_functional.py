@@ -145,6 +145,27 @@ def test_a_class_keeps_a_forward_that_it_was_given(monkeypatch, kind, shape):
     assert torch.equal(early(t), want)
 
 
+@pytest.mark.parametrize('kind,shape', [(nn.LayerNorm, (8, )), (nn.Embedding, (10, 8))])
+def test_a_class_keeps_a_forward_that_it_had_before_the_import(monkeypatch, kind, shape):
+    import functools
+    import importlib.util
+    import elixir_b200.functional as F
+    torch_forward = kind.forward
+
+    @functools.wraps(torch_forward)
+    def patched(layer, t):
+        return 2 * torch_forward(layer, t)
+
+    monkeypatch.setattr(kind, 'forward', patched)
+    spec = importlib.util.spec_from_file_location('elixir_b200._imported_late', F.__file__)
+    late = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(late)
+    layer = kind(*shape)
+    assert late.use_kernels(layer) == 0 and 'forward' not in layer.__dict__
+    monkeypatch.undo()
+    assert late._torch_forward(kind) is torch_forward and F._TORCH_FORWARD[kind] is torch_forward
+
+
 def test_layers_leave_fake_tensors_and_subclasses_to_torch(monkeypatch):
     """A fake CUDA tensor has no memory that a kernel could take."""
     from torch._subclasses.fake_tensor import FakeTensorMode
